@@ -46,6 +46,15 @@ class DensePlan:
         s.res_nnz, s.res_max_row = self.res_indices.numel(), self.res_max_row
         self.struct = s
         self.ref = ctypes.byref(s)
+        self._workspace_bytes = {}
+
+    def workspace_bytes(self, F):
+        """Scratch a call at width F needs.  Kept on the plan itself: a table keyed by the plan's id would answer for
+        a later plan that the allocator put at the same address."""
+        n = self._workspace_bytes.get(F)
+        if n is None:
+            n = self._workspace_bytes[F] = _lib.lib().tango_spmm_dense_workspace(self.ref, F)
+        return n
 
 
 # what a segment costs beside its units, in units of work: its prologue and flush; the atomic flush of a shared block

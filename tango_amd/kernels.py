@@ -610,10 +610,7 @@ class cuda_kernels:
             _need(scale_mul, torch.float32, "scale_mul")
             if scale_mul.numel() != plan.rows or scale_out is None:
                 raise RuntimeError("csr_SPMM_dense: scale_mul needs one entry per output row and a scale_out")
-        key = ("dense", id(plan), F)
-        ws_bytes = _WS_SIZES.get(key)
-        if ws_bytes is None:
-            ws_bytes = _WS_SIZES[key] = _L.tango_spmm_dense_workspace(plan.ref, F)
+        ws_bytes = plan.workspace_bytes(F)
         ws = _workspace(ws_bytes, U.device)
         check(_L.tango_spmm_csr_copy_u_dense(_ptr(out), plan.ref, _ptr(U), ldf, scaleU.data_ptr(), _ptr(row_scale),
                                              _ptr(bias), int(bool(relu)), _ptr(sign_bits), F, _ptr(scale_mul),
