@@ -43,6 +43,9 @@ enum tango_round_mode {
 
 enum tango_sddmm_op { TANGO_OP_ADD = 0, TANGO_OP_SUB = 1, TANGO_OP_MUL = 2, TANGO_OP_DIV = 3 };
 
+/* Element types of the entry points that take more than fp32. */
+enum tango_dtype { TANGO_F32 = 0, TANGO_BF16 = 1, TANGO_F16 = 2 };
+
 const char* tango_status_string(int status);
 /* ABI version; bumped when a signature changes. */
 int tango_abi_version(void);
@@ -593,6 +596,59 @@ int tango_batchnorm_bwd_f32(float* dx, float* dgamma, float* dbeta, const float*
                             const float* gamma, const float* beta, int64_t rows, int64_t cols,
                             int relu, void* workspace, size_t workspace_bytes,
                             tango_stream_t stream);
+
+/* ---- 8-bit checkpoints of activations (no counterpart in the reference) --------------------
+   x [rows, cols] (dtype: a tango_dtype) as int8 plus one fp32 scale per run of `group` consecutive columns of a row;
+   the last run of a row may be shorter, group >= cols gives one run a row.  Per run
+     scale = max|x| / 127 (at most the largest whose 127-fold is finite),  q = the integer nearest to 127 x / max|x|, ties to even (decided exactly),
+   and q * scale is the value held.  A run with an infinity or a NaN gets scale NaN and q = 0 (every value of it comes
+   back as NaN); a run of zeros gets scale 0.  scale: [rows, ceil(cols / group)], contiguous.  Rows that start on
+   16-byte multiples and runs that are a multiple of 16 bytes take the widest loads; anything else is taken too. */
+int tango_pack_i8(int8_t* q, int64_t ldq, float* scale, const void* x, int dtype, int64_t rows,
+                  int64_t cols, int64_t ldx, int64_t group, tango_stream_t stream);
+/* x[r, c] = q[r, c] * scale[r, c / group] in fp32, then rounded to dtype. */
+int tango_unpack_i8(void* x, int dtype, int64_t ldx, const int8_t* q, int64_t ldq, const float* scale,
+                    int64_t rows, int64_t cols, int64_t group, tango_stream_t stream);
+
+/* ---- Softmax attention over a graph's edges (no counterpart in the reference, which runs an SDDMM, an edge
+   softmax and an SpMM with a value per edge and head between them) --------------------------
+     out[d, h] = sum_e p_e v[s_e, h'],  p = softmax over the in-edges e = (s_e -> d) of d of scale * (q[d, h] . k[s_e, h']),
+   h' = h / (heads / kv_heads).  A destination without an edge that takes part gets zeros. */
+typedef struct tango_attention {
+    int64_t num_dst, num_src, heads, kv_heads, dim; /* heads a multiple of kv_heads; dim <= 256 */
+    int dtype;                                      /* tango_dtype of out, dout and the gradients; without checkpoint also of q, k, v */
+    int checkpoint;                                 /* backward only: q, k, v are int8 with the scales below */
+    const void *q, *k, *v;                          /* element (r, h, i) at r * row + h * head + i */
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    const float *q_scale, *k_scale, *v_scale;       /* [rows, heads of the tensor]: a tango_pack_i8 with group = dim */
+    float scale;
+} tango_attention;
+
+/* The rows of one orientation (destinations with their in-edges, or sources with their out-edges) as work items. */
+typedef struct tango_attn_items {
+    int64_t num_items, num_parts, num_split, num_edges;
+    const int32_t* items;    /* [num_items, 4]: row, first slot, last slot + 1, part or -1.  Every row is one item (part
+                                -1) or several, whose parts are consecutive and in slot order; 16-byte aligned */
+    const int32_t* split;    /* [num_split, 4]: a row of several items, its first part, its last part + 1, 0 */
+    const int32_t* indices;  /* [num_edges]: the other endpoint of a slot's edge */
+    const int32_t* edge_ids; /* [num_edges] or NULL (a slot's number is its edge's id): what edge_mask is indexed by */
+} tango_attn_items;
+
+/* Bytes of scratch for the forward pass (by_src NULL) or the backward pass. */
+size_t tango_graph_attention_workspace(const tango_attention* t, const tango_attn_items* by_dst,
+                                       const tango_attn_items* by_src);
+/* out [num_dst, heads, dim] contiguous.  edge_mask: [num_edges] bytes by edge id, 0 = the edge takes no part (whatever
+   its key and value hold); NULL: all do.  With checkpoint set: TANGO_ERR_UNSUPPORTED. */
+int tango_graph_attention_fwd(void* out, const tango_attention* t, const tango_attn_items* by_dst,
+                              const uint8_t* edge_mask, void* workspace, size_t workspace_bytes,
+                              tango_stream_t stream);
+/* Gradients for dout (strides in elements, unit last stride) at the q, k, v of `t`, or at what its checkpoints hold;
+   the probabilities are formed again.  dq [num_dst, heads, dim], dk and dv [num_src, kv_heads, dim], contiguous; each
+   may be NULL.  All sums run in a fixed order. */
+int tango_graph_attention_bwd(void* dq, void* dk, void* dv, const tango_attention* t, const void* dout,
+                              int64_t dout_row, int64_t dout_head, const tango_attn_items* by_dst,
+                              const tango_attn_items* by_src, const uint8_t* edge_mask, void* workspace,
+                              size_t workspace_bytes, tango_stream_t stream);
 
 #ifdef __cplusplus
 }

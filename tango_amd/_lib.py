@@ -77,6 +77,11 @@ SIGNATURES = {
     "tango_edge_softmax_fwd_ex": (I, [P, P, P, P, P, P, P, P, P, P, P, P, I64, I64, I64, F, P, SZ, P]),
     "tango_edge_softmax_bwd_ex": (I, [P, P, P, P, P, P, P, P, I64, I64, I64, F, P, SZ, P]),
     "tango_edge_softmax_bwd": (I, [P, P, P, P, P, P, I64, I64, I64, F, P, SZ, P]),
+    "tango_pack_i8": (I, [P, I64, P, P, I, I64, I64, I64, I64, P]),
+    "tango_unpack_i8": (I, [P, I, I64, P, I64, P, I64, I64, I64, P]),
+    "tango_graph_attention_workspace": (SZ, [P, P, P]),
+    "tango_graph_attention_fwd": (I, [P, P, P, P, P, SZ, P]),
+    "tango_graph_attention_bwd": (I, [P, P, P, P, P, I64, I64, P, P, P, P, SZ, P]),
 }
 
 
@@ -88,6 +93,20 @@ class DensePlan(C.Structure):
                [(n, P) for n in ("col_ids", "row_slot", "row_order", "mask_off", "mask", "seg_ptr", "segs", "seg_ptr2", "segs2", "shared_blocks",
                                  "res_indptr", "res_indices")] + \
                [("res_nnz", I64), ("res_max_row", I64)]
+
+
+class Attention(C.Structure):
+    """tango_attention of include/tango_hip.h."""
+    _fields_ = [(n, I64) for n in ("num_dst", "num_src", "heads", "kv_heads", "dim")] + \
+               [("dtype", I), ("checkpoint", I)] + [(n, P) for n in ("q", "k", "v")] + \
+               [(n, I64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")] + \
+               [(n, P) for n in ("q_scale", "k_scale", "v_scale")] + [("scale", F)]
+
+
+class AttnItems(C.Structure):
+    """tango_attn_items of include/tango_hip.h."""
+    _fields_ = [(n, I64) for n in ("num_items", "num_parts", "num_split", "num_edges")] + \
+               [(n, P) for n in ("items", "split", "indices", "edge_ids")]
 
 
 ROUND_RNE, ROUND_TRUNC, ROUND_STOCHASTIC = 0, 1, 2

@@ -1,0 +1,190 @@
+// C entries of the attention over a graph's edges: checks, workspace layout, the order of the passes.  The kernels are
+// in graph_attention.hpp.
+#include "graph_attention.hpp"
+
+namespace tango {
+
+extern template bool launch_attention<float, float>(AttnPass, AttnArgs, JoinArgs, int64_t, bool, hipStream_t);
+extern template bool launch_attention<bf16_t, bf16_t>(AttnPass, AttnArgs, JoinArgs, int64_t, bool, hipStream_t);
+extern template bool launch_attention<f16_t, f16_t>(AttnPass, AttnArgs, JoinArgs, int64_t, bool, hipStream_t);
+extern template bool launch_attention<int8_t, float>(AttnPass, AttnArgs, JoinArgs, int64_t, bool, hipStream_t);
+extern template bool launch_attention<int8_t, bf16_t>(AttnPass, AttnArgs, JoinArgs, int64_t, bool, hipStream_t);
+extern template bool launch_attention<int8_t, f16_t>(AttnPass, AttnArgs, JoinArgs, int64_t, bool, hipStream_t);
+
+static bool launch_any(const tango_attention& t, AttnPass pass, const AttnArgs& a, const JoinArgs& j, int64_t num_split,
+                       bool aligned, hipStream_t s) {
+    if (t.checkpoint) {
+        if (t.dtype == TANGO_F32) return launch_attention<int8_t, float>(pass, a, j, num_split, aligned, s);
+        if (t.dtype == TANGO_BF16) return launch_attention<int8_t, bf16_t>(pass, a, j, num_split, aligned, s);
+        return launch_attention<int8_t, f16_t>(pass, a, j, num_split, aligned, s);
+    }
+    if (t.dtype == TANGO_F32) return launch_attention<float, float>(pass, a, j, num_split, aligned, s);
+    if (t.dtype == TANGO_BF16) return launch_attention<bf16_t, bf16_t>(pass, a, j, num_split, aligned, s);
+    return launch_attention<f16_t, f16_t>(pass, a, j, num_split, aligned, s);
+}
+
+static int check_shape(const tango_attention* t) {
+    if (!t) return TANGO_ERR_INVALID_ARG;
+    if (!float_type(t->dtype)) return TANGO_ERR_UNSUPPORTED;
+    if (t->num_dst < 0 || t->num_src < 0 || t->heads <= 0 || t->kv_heads <= 0 || t->dim <= 0) return TANGO_ERR_INVALID_ARG;
+    if (t->num_dst >= (1LL << 31) || t->num_src >= (1LL << 31) || t->heads > 65536 || t->heads % t->kv_heads || t->dim > 256)
+        return TANGO_ERR_UNSUPPORTED;
+    return TANGO_OK;
+}
+
+static int check_items(const tango_attn_items* i, int64_t rows) {
+    if (!i || i->num_items < 0 || i->num_parts < 0 || i->num_split < 0 || i->num_edges < 0) return TANGO_ERR_INVALID_ARG;
+    if (i->num_edges > (1LL << 31) - 4096 || i->num_parts >= (1LL << 31)) return TANGO_ERR_UNSUPPORTED;
+    if (i->num_items < rows || i->num_split > i->num_parts) return TANGO_ERR_INVALID_ARG;  // every row is at least one item
+    if ((i->num_items && (!i->items || !aligned_to(i->items, 16))) || (i->num_split && (!i->split || !aligned_to(i->split, 16))))
+        return TANGO_ERR_INVALID_ARG;
+    if (i->num_edges && !i->indices) return TANGO_ERR_INVALID_ARG;
+    return TANGO_OK;
+}
+
+static int64_t align256(int64_t b) { return (b + 255) & ~255LL; }
+
+static int64_t forward_part_bytes(const tango_attention& t, const tango_attn_items& i) {
+    return align256(i.num_parts * t.heads * (t.dim + 2) * 4);
+}
+static int64_t stats_bytes(const tango_attention& t) { return align256(t.num_dst * t.heads * 8); }
+static int64_t backward_part_bytes(const tango_attention& t, const tango_attn_items& d, const tango_attn_items& s) {
+    const int64_t a = align256(d.num_parts * t.heads * (2 * t.dim + 3) * 4), b = align256(s.num_parts * t.kv_heads * 2 * t.dim * 4);
+    return a > b ? a : b;
+}
+
+static int check_operands(const tango_attention& t) {
+    if ((t.num_dst && !t.q) || (t.num_src && (!t.k || !t.v))) return TANGO_ERR_INVALID_ARG;
+    if (t.checkpoint && ((t.num_dst && !t.q_scale) || (t.num_src && (!t.k_scale || !t.v_scale)))) return TANGO_ERR_INVALID_ARG;
+    const int64_t size = t.checkpoint ? 1 : element_size(t.dtype);
+    if (!aligned_to(t.q, size) || !aligned_to(t.k, size) || !aligned_to(t.v, size)) return TANGO_ERR_INVALID_ARG;
+    return TANGO_OK;
+}
+
+// Whether a lane's pieces of `size`-byte elements can be loaded whole.
+static bool rows_aligned(const void* p, int64_t row, int64_t head, int64_t vec, int64_t size) {
+    const int64_t bytes = vec * size < 16 ? vec * size : 16;
+    return aligned_to(p, bytes) && row * size % bytes == 0 && head * size % bytes == 0;
+}
+
+static void fill_args(AttnArgs& a, const tango_attention& t) {
+    a = AttnArgs();
+    a.q = t.q;
+    a.k = t.k;
+    a.v = t.v;
+    a.q_scale = t.q_scale;
+    a.k_scale = t.k_scale;
+    a.v_scale = t.v_scale;
+    a.q_row = t.q_row;
+    a.q_head = t.q_head;
+    a.k_row = t.k_row;
+    a.k_head = t.k_head;
+    a.v_row = t.v_row;
+    a.v_head = t.v_head;
+    a.heads = static_cast<int>(t.heads);
+    a.kv_heads = static_cast<int>(t.kv_heads);
+    a.rep = a.heads / a.kv_heads;
+    a.dim = static_cast<int>(t.dim);
+    a.scale = t.scale;
+}
+
+static void use_items(AttnArgs& a, JoinArgs& j, const tango_attn_items& i, const uint8_t* mask, int heads) {
+    a.items = reinterpret_cast<const int4*>(i.items);
+    a.num_items = i.num_items;
+    a.indices = i.indices;
+    a.edge_ids = i.edge_ids;
+    a.mask = mask;
+    j.split = reinterpret_cast<const int4*>(i.split);
+    j.parts = a.parts;
+    j.out = a.out;
+    j.out2 = a.out2;
+    j.stats = a.stats;
+    j.heads = heads;
+    j.dim = a.dim;
+    j.width = 1;
+    while (j.width < a.dim) j.width <<= 1;
+    j.scale = a.scale;
+}
+
+}  // namespace tango
+
+using namespace tango;
+
+extern "C" {
+
+size_t tango_graph_attention_workspace(const tango_attention* t, const tango_attn_items* by_dst, const tango_attn_items* by_src) {
+    if (check_shape(t) != TANGO_OK || !by_dst) return 0;
+    if (!by_src) return static_cast<size_t>(forward_part_bytes(*t, *by_dst));
+    return static_cast<size_t>(stats_bytes(*t) + backward_part_bytes(*t, *by_dst, *by_src));
+}
+
+int tango_graph_attention_fwd(void* out, const tango_attention* t, const tango_attn_items* by_dst, const uint8_t* edge_mask,
+                              void* workspace, size_t workspace_bytes, tango_stream_t stream) {
+    int rc = check_shape(t);
+    if (rc == TANGO_OK) rc = check_items(by_dst, t->num_dst);
+    if (rc == TANGO_OK) rc = check_operands(*t);
+    if (rc != TANGO_OK) return rc;
+    if (t->checkpoint) return TANGO_ERR_UNSUPPORTED;  // the forward pass runs on the tensors themselves
+    if (t->num_dst == 0) return TANGO_OK;
+    if (!out || (by_dst->num_edges && t->num_src == 0)) return TANGO_ERR_INVALID_ARG;
+    const int64_t need = forward_part_bytes(*t, *by_dst);
+    if (need && (!workspace || static_cast<int64_t>(workspace_bytes) < need || !aligned_to(workspace, 16))) return TANGO_ERR_WORKSPACE;
+    AttnArgs a;
+    JoinArgs j = JoinArgs();
+    fill_args(a, *t);
+    a.out = out;
+    a.parts = static_cast<float*>(workspace);
+    use_items(a, j, *by_dst, edge_mask, a.heads);
+    const int64_t size = element_size(t->dtype), vec = size == 4 ? 4 : 8;
+    const bool aligned = t->dim % vec == 0 && rows_aligned(t->q, t->q_row, t->q_head, vec, size) &&
+                         rows_aligned(t->k, t->k_row, t->k_head, vec, size) && rows_aligned(t->v, t->v_row, t->v_head, vec, size) &&
+                         aligned_to(out, 16);
+    if (!launch_any(*t, kPassForward, a, j, by_dst->num_split, aligned, as_stream(stream))) return TANGO_ERR_UNSUPPORTED;
+    return launch_status();
+}
+
+int tango_graph_attention_bwd(void* dq, void* dk, void* dv, const tango_attention* t, const void* dout, int64_t dout_row,
+                              int64_t dout_head, const tango_attn_items* by_dst, const tango_attn_items* by_src,
+                              const uint8_t* edge_mask, void* workspace, size_t workspace_bytes, tango_stream_t stream) {
+    int rc = check_shape(t);
+    if (rc == TANGO_OK) rc = check_items(by_dst, t->num_dst);
+    if (rc == TANGO_OK) rc = check_items(by_src, t->num_src);
+    if (rc == TANGO_OK) rc = check_operands(*t);
+    if (rc != TANGO_OK) return rc;
+    if (by_dst->num_edges != by_src->num_edges || (t->num_dst && !dout)) return TANGO_ERR_INVALID_ARG;
+    if (by_dst->num_edges && (t->num_src == 0 || t->num_dst == 0)) return TANGO_ERR_INVALID_ARG;
+    if (!dq && !dk && !dv) return TANGO_OK;
+    const int64_t need = stats_bytes(*t) + backward_part_bytes(*t, *by_dst, *by_src);
+    if (need && (!workspace || static_cast<int64_t>(workspace_bytes) < need || !aligned_to(workspace, 16))) return TANGO_ERR_WORKSPACE;
+    const int64_t size = t->checkpoint ? 1 : element_size(t->dtype), vec = size == 4 ? 4 : 8;
+    const int64_t gsize = element_size(t->dtype);
+    const bool aligned = t->dim % vec == 0 && rows_aligned(t->q, t->q_row, t->q_head, vec, size) &&
+                         rows_aligned(t->k, t->k_row, t->k_head, vec, size) && rows_aligned(t->v, t->v_row, t->v_head, vec, size) &&
+                         rows_aligned(dout, dout_row, dout_head, vec, gsize) && aligned_to(dq, 16) && aligned_to(dk, 16) &&
+                         aligned_to(dv, 16);
+    AttnArgs a;
+    JoinArgs j = JoinArgs();
+    fill_args(a, *t);
+    a.dout = dout;
+    a.do_row = dout_row;
+    a.do_head = dout_head;
+    a.stats = static_cast<float2*>(workspace);
+    a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(*t));
+    if (t->num_dst) {
+        a.out = dq;
+        use_items(a, j, *by_dst, edge_mask, a.heads);
+        if (!launch_any(*t, kPassQuery, a, j, by_dst->num_split, aligned, as_stream(stream))) return TANGO_ERR_UNSUPPORTED;
+        rc = launch_status();
+        if (rc != TANGO_OK) return rc;
+    }
+    if (t->num_src && (dk || dv)) {
+        a.out = dk;
+        a.out2 = dv;
+        use_items(a, j, *by_src, edge_mask, a.kv_heads);
+        if (!launch_any(*t, kPassKeyValue, a, j, by_src->num_split, aligned, as_stream(stream))) return TANGO_ERR_UNSUPPORTED;
+        rc = launch_status();
+    }
+    return rc;
+}
+
+}  // extern "C"

@@ -1,0 +1,93 @@
+"""Refusals of the checkpoint and attention entry points that need no GPU: everything is checked on the host before
+anything is launched, so the made-up pointers are never followed."""
+import ctypes
+
+import pytest
+import torch
+
+
+def test_python_refusals():
+    from tango_amd.checkpoint import pack
+    from tango_amd.graph_attention import graph_attention
+    with pytest.raises(RuntimeError, match="GPU"):
+        pack(torch.zeros(4, 8))
+    with pytest.raises(TypeError):
+        pack([1.0])
+    with pytest.raises(RuntimeError, match="GPU"):
+        graph_attention(None, *(torch.zeros(2, 1, 4) for _ in range(3)))
+
+
+def test_checkpoint_abi_refusals():
+    from tango_amd import _lib
+    L = _lib.lib()
+    assert L.tango_pack_i8(16, 8, 16, 16, 3, 4, 8, 8, 8, None) == -2   # no such type
+    assert L.tango_pack_i8(16, 8, 16, 16, 0, -1, 8, 8, 8, None) == -1
+    assert L.tango_pack_i8(16, 8, 16, 16, 0, 4, 8, 8, 0, None) == -1   # group
+    assert L.tango_pack_i8(16, 8, 16, None, 0, 4, 8, 8, 8, None) == -1
+    assert L.tango_pack_i8(16, 4, 16, 16, 0, 4, 8, 8, 8, None) == -1   # rows of the result overlap
+    assert L.tango_pack_i8(16, 8, 16, 18, 0, 4, 8, 8, 8, None) == -1   # fp32 off its alignment
+    assert L.tango_pack_i8(16, 8, 16, 16, 0, 4, 1 << 30, 1 << 30, 8, None) == -2
+    assert L.tango_pack_i8(None, 8, None, None, 0, 0, 8, 8, 8, None) == 0
+    assert L.tango_unpack_i8(16, 0, 4, 16, 8, 16, 4, 8, 8, None) == -1
+    assert L.tango_unpack_i8(16, 7, 8, 16, 8, 16, 4, 8, 8, None) == -2
+    assert L.tango_unpack_i8(None, 0, 8, None, 8, None, 4, 0, 8, None) == 0
+
+
+def _attention(**kw):
+    from tango_amd import _lib
+    t = _lib.Attention(num_dst=4, num_src=4, heads=2, kv_heads=2, dim=8, q=16, k=16, v=16, q_row=16, q_head=8, k_row=16,
+                       k_head=8, v_row=16, v_head=8, scale=1.0)
+    i = _lib.AttnItems(num_items=4, num_edges=5, items=16, indices=16)
+    for name, value in kw.items():
+        setattr(i if hasattr(i, name) else t, name, value)
+    return _lib.lib(), t, i
+
+
+@pytest.mark.parametrize("status,change", [
+    (-2, {"dtype": 3}), (-1, {"dim": 0}), (-2, {"dim": 257}), (-1, {"heads": 0}), (-2, {"heads": 3}), (-1, {"num_dst": -1}),
+    (-2, {"num_src": 1 << 31}), (-1, {"q": None}), (-1, {"k": 18}), (-2, {"checkpoint": 1, "q_scale": 16, "k_scale": 16, "v_scale": 16}),
+    (-1, {"checkpoint": 1}), (-1, {"num_items": 3}), (-1, {"items": 20}), (-1, {"indices": None}), (-2, {"num_edges": 1 << 31}),
+    (-1, {"num_split": 1, "num_parts": 2, "split": None}), (-4, {"num_split": 1, "num_parts": 2, "split": 16}), (-1, {"num_src": 0}),
+])
+def test_attention_abi_refusals(status, change):
+    L, t, i = _attention(**change)
+    assert L.tango_graph_attention_fwd(16, ctypes.byref(t), ctypes.byref(i), None, None, 0, None) == status
+
+
+def test_attention_backward_abi_refusals():
+    L, t, i = _attention()
+    refs = ctypes.byref(t), ctypes.byref(i)
+    assert L.tango_graph_attention_bwd(16, 16, 16, refs[0], None, 16, 8, refs[1], refs[1], None, None, 0, None) == -1
+    assert L.tango_graph_attention_bwd(16, 16, 16, refs[0], 16, 16, 8, refs[1], None, None, None, 0, None) == -1
+    assert L.tango_graph_attention_bwd(16, 16, 16, refs[0], 16, 16, 8, refs[1], refs[1], None, None, 0, None) == -4
+    assert L.tango_graph_attention_bwd(None, None, None, refs[0], 16, 16, 8, refs[1], refs[1], None, None, 0, None) == 0
+    assert L.tango_graph_attention_fwd(None, refs[0], refs[1], None, None, 0, None) == -1
+    assert L.tango_graph_attention_workspace(refs[0], refs[1], None) == 0  # no row is cut
+    assert L.tango_graph_attention_workspace(refs[0], refs[1], refs[1]) >= 4 * 2 * 8  # two floats a destination and head
+
+
+@pytest.mark.parametrize("cap", [1, 3, 64])
+def test_items_cover_every_edge_once(cap):
+    """The cut into items: every slot once, rows in slot order, no item longer than the cap, empty rows present."""
+    from tango_amd.graph_attention import AttentionItems
+    degree = torch.tensor([0, 1, 200, 0, 64, 65, 3, 0, 129, 2])
+    indptr = torch.zeros(11, dtype=torch.int64)
+    indptr[1:] = torch.cumsum(degree, 0)
+    a = AttentionItems(indptr, torch.zeros(int(indptr[-1]), dtype=torch.int32), None, cap=cap)
+    items = a.items.tolist()
+    lengths = [last - first for _, first, last, _ in items]
+    assert lengths == sorted(lengths, reverse=True) and max(lengths) <= cap
+    seen = torch.zeros(int(indptr[-1]), dtype=torch.int64)
+    for row, first, last, part in items:
+        assert indptr[row] <= first <= last <= indptr[row + 1]
+        seen[first:last] += 1
+    assert (seen == 1).all() and sorted({r for r, _, _, _ in items}) == list(range(10))
+    cut = {row: (a0, a1) for row, a0, a1, _ in a.split.tolist()}
+    for row in range(10):
+        mine = sorted(i for i in items if i[0] == row)
+        if row not in cut:
+            assert len(mine) == 1 and mine[0][3] == -1
+        else:
+            assert [i[3] for i in mine] == list(range(*cut[row])) and mine[0][1] == indptr[row] and mine[-1][2] == indptr[row + 1]
+            assert all(x[2] == y[1] for x, y in zip(mine, mine[1:]))
+    assert a.struct.num_parts == sum(b - c for c, b in cut.values())
