@@ -610,6 +610,17 @@ int tango_pack_i8(int8_t* q, int64_t ldq, float* scale, const void* x, int dtype
 int tango_unpack_i8(void* x, int dtype, int64_t ldx, const int8_t* q, int64_t ldq, const float* scale,
                     int64_t rows, int64_t cols, int64_t group, tango_stream_t stream);
 
+/* Gradients of a linear layer's weight and bias from the 8-bit checkpoint of its input (q, scale, group as
+   tango_pack_i8 wrote them; ldq a multiple of 4 is the fast case):
+     dw[n, k] = sum_m dy[m, n] * (q[m, k] * scale[m, k / group]),   db[n] = sum_m dy[m, n]  (db may be NULL)
+   for dy [M, N] (dtype, row stride ldy) and q [M, K]; dw [N, K] and db [N] in dtype, contiguous.  Sums are fp32 in a
+   fixed order; a row's dy * scale is held in three (fp32) or two (bf16, fp16) bf16 terms.  A dy that is not finite
+   gives a result that is not finite.  workspace: tango_weight_grad_i8_workspace bytes. */
+size_t tango_weight_grad_i8_workspace(int64_t M, int64_t N, int64_t K, int64_t group);
+int tango_weight_grad_i8(void* dw, void* db, const void* dy, int dtype, int64_t ldy, const int8_t* q,
+                         int64_t ldq, const float* scale, int64_t group, int64_t M, int64_t N, int64_t K,
+                         void* workspace, size_t workspace_bytes, tango_stream_t stream);
+
 /* ---- Softmax attention over a graph's edges (no counterpart in the reference, which runs an SDDMM, an edge
    softmax and an SpMM with a value per edge and head between them) --------------------------
      out[d, h] = sum_e p_e v[s_e, h'],  p = softmax over the in-edges e = (s_e -> d) of d of scale * (q[d, h] . k[s_e, h']),

@@ -13,7 +13,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libtango_hip.so")
 SOURCES = ["quantize.hip", "spmm.hip", "spmm_dense.hip", "sddmm.hip", "edge_softmax.hip", "qgemm.hip", "loss.hip", "attention.hip", "batchnorm.hip",
-           "checkpoint.hip", "graph_attention.hip", "graph_attention_f32.hip", "graph_attention_bf16.hip", "graph_attention_f16.hip"]
+           "checkpoint.hip", "weight_grad.hip", "graph_attention.hip", "graph_attention_f32.hip", "graph_attention_bf16.hip", "graph_attention_f16.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

@@ -7,12 +7,20 @@ of small values is not held at the resolution of the largest row.
 
     p = pack(x, group=32)                       # int8 values + fp32 scales: 1.125 bytes an element
     y = unpack(p)                               # the values it holds, in x's type
+    dw, db = weight_grad(dy, p, want_bias=True) # of a linear layer whose input x was, without restoring x
+
+``CheckpointLinear`` is a linear layer that keeps its input that way; ``tango_amd.graph_attention`` keeps queries, keys
+and values that way when asked to.
 """
 import contextlib
+import math
 
 import torch
+import torch.nn as nn
+import torch.nn.functional as F
+from torch.autograd.function import Function, once_differentiable
 
-from .kernels import _L, _current_device, _ptr, _stream, check
+from .kernels import _L, _current_device, _ptr, _stream, _workspace, check, refuse_capture
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # tango_dtype of include/tango_hip.h
 
@@ -53,7 +61,7 @@ class Packed:
 def _rows_of(x):
     """[rows, cols] with contiguous columns: a view where x's layout allows one."""
     cols = x.size(-1)
-    rows = x.numel() // cols if cols else 0
+    rows = math.prod(x.shape[:-1])
     if cols > 1 and x.stride(-1) != 1:
         x = x.contiguous()
     return x.reshape(rows, cols)
@@ -97,3 +105,79 @@ def unpack(packed, dtype=None):
         check(_L.tango_unpack_i8(_ptr(out), DTYPES[dtype], cols, _ptr(packed.values), packed.values.stride(0),
                                  _ptr(packed.scale), rows, cols, packed.group, _stream()), "unpack")
     return out
+
+
+def weight_grad(dy, packed, want_bias=False):
+    """``dy.T @ x`` (and, with ``want_bias``, ``dy.sum(0)``) for the x that ``packed`` holds: the gradients of a linear
+    layer's weight [out, in] and bias from the gradient ``dy`` [..., out] of its output, in dy's type, read straight
+    from the 8-bit values.  Sums are fp32 in a fixed order."""
+    need_float(dy, "dy")
+    if not isinstance(packed, Packed):
+        raise TypeError("weight_grad: expected what pack returned")
+    if dy.dim() < 1 or dy.device != packed.device:
+        raise RuntimeError("weight_grad: dy must be [..., out] on the checkpoint's device")
+    rows, cols = packed.values.shape
+    n = dy.size(-1)
+    if math.prod(dy.shape[:-1]) != rows:
+        raise RuntimeError("weight_grad: dy needs a row for each of the checkpoint's %d" % rows)
+    with on_device_of(dy):
+        flat = _rows_of(dy.detach())
+        if rows == 0:
+            dw, db = flat.new_zeros((n, cols)), flat.new_zeros(n)
+        else:
+            dw = torch.empty((n, cols), dtype=dy.dtype, device=dy.device)
+            db = torch.empty(n, dtype=dy.dtype, device=dy.device) if want_bias else None
+            if cols == 0 and want_bias:
+                db = flat.float().sum(0).to(dy.dtype)
+            ws_bytes = _L.tango_weight_grad_i8_workspace(rows, n, cols, packed.group)
+            ws = _workspace(ws_bytes, dy.device)
+            check(_L.tango_weight_grad_i8(_ptr(dw), _ptr(db) if want_bias else None, _ptr(flat), DTYPES[dy.dtype],
+                                          flat.stride(0) if rows > 1 else n, _ptr(packed.values), packed.values.stride(0),
+                                          _ptr(packed.scale), packed.group, rows, n, cols, _ptr(ws), ws_bytes, _stream()),
+                  "weight_grad")
+    return (dw, db) if want_bias else dw
+
+
+class checkpoint_linear(Function):
+    """``x @ weight.T + bias`` on the tensors themselves, keeping x in 8 bits (``pack(x, group)``) for the weight's
+    gradient.  The input's gradient dy @ weight does not need x."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, group=None):
+        for t, name in ((x, "x"), (weight, "weight")) + (((bias, "bias"),) if bias is not None else ()):
+            need_float(t, name)
+            if t.dtype != x.dtype or t.device != x.device:
+                raise RuntimeError("checkpoint_linear: %s must have x's type and device" % name)
+        ctx.has_bias = bias is not None
+        ctx.held = pack(x, group) if ctx.needs_input_grad[1] else None
+        ctx.save_for_backward(weight if ctx.needs_input_grad[0] else None)
+        return F.linear(x, weight, bias)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        refuse_capture("checkpoint_linear.backward")
+        weight, = ctx.saved_tensors
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        dx = torch.matmul(dy, weight) if want_x else None
+        dw = db = None
+        if want_w:
+            dw, db = weight_grad(dy, ctx.held, True) if want_b else (weight_grad(dy, ctx.held), None)
+        elif want_b:
+            db = dy.float().reshape(-1, dy.size(-1)).sum(0).to(dy.dtype)
+        return dx, dw, db, None
+
+
+class CheckpointLinear(nn.Linear):
+    """``nn.Linear`` (same parameters and state dict) whose input is held in 8 bits between the passes, with a scale
+    per run of ``group`` columns of a row (None: one a row).  Beside ``QLinear``: the forward pass and the input's
+    gradient are not quantized, only what the weight's gradient reads is."""
+
+    def __init__(self, in_features, out_features, bias=True, group=None, **kw):
+        super().__init__(in_features, out_features, bias, **kw)
+        if group is not None and (int(group) != group or group < 1):
+            raise ValueError("CheckpointLinear: group must be a positive whole number of columns")
+        self.group = group
+
+    def forward(self, x):
+        return checkpoint_linear.apply(x, self.weight, self.bias, self.group)

@@ -33,6 +33,19 @@ def test_checkpoint_abi_refusals():
     assert L.tango_unpack_i8(None, 0, 8, None, 8, None, 4, 0, 8, None) == 0
 
 
+def test_weight_grad_abi_refusals():
+    from tango_amd import _lib
+    L = _lib.lib()
+    ok = dict(dw=16, db=None, dy=16, dtype=0, ldy=8, q=16, ldq=16, scale=16, group=16, M=4, N=8, K=16, ws=None, nbytes=0, stream=None)
+    call = lambda **kw: L.tango_weight_grad_i8(*{**ok, **kw}.values())
+    assert call() == -4 and call(ws=16, nbytes=8) == -4
+    assert call(dtype=5) == -2 and call(N=1 << 17) == -2 and call(M=1 << 31) == -2
+    assert call(M=0) == -1 and call(group=0) == -1 and call(dy=None) == -1 and call(dw=18) == -1 and call(scale=None) == -1
+    assert call(N=0) == 0 and call(K=0) == 0
+    assert L.tango_weight_grad_i8_workspace(4, 8, 16, 16) >= 4 * (8 * 16 + 8)
+    assert L.tango_weight_grad_i8_workspace(0, 8, 16, 16) == 0
+
+
 def _attention(**kw):
     from tango_amd import _lib
     t = _lib.Attention(num_dst=4, num_src=4, heads=2, kv_heads=2, dim=8, q=16, k=16, v=16, q_row=16, q_head=8, k_row=16,

@@ -3,6 +3,8 @@
 The integers are decided in 64 bits: 127 x is exact there (at most 31 bits), a quotient that is a tie is exact, and one
 that is not differs from a tie by more than 2^-40 of itself, far more than a 64-bit division's rounding.  So integers
 must be equal, scales are one fp32 division (equal), and a restored value is one product and one rounding (equal)."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -39,7 +41,7 @@ def compare(x, group):
     from tango_amd.checkpoint import pack, unpack
     cols = x.size(-1)
     p = pack(x, group)
-    q, scale = expected(x.reshape(x.numel() // cols if cols else 0, cols), group or max(cols, 1))
+    q, scale = expected(x.reshape(math.prod(x.shape[:-1]), cols), group or max(cols, 1))
     assert p.values.dtype == torch.int8 and p.values.shape == q.shape
     assert np.array_equal(host(p.values), q)
     assert np.array_equal(host(p.scale), scale, equal_nan=True)
