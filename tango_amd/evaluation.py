@@ -20,6 +20,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .checkpoint import CheckpointLinear
 from .gat import GAT, HGT, ArxivGAT, HeteroHGTLayer, QGATConv, relation_graphs, relation_major
 from .gcn import GCN, ArxivGCN
 from .graph import Graph, add_self_loop, chung_lu, hetero_power_law, remove_self_loop
@@ -194,9 +195,10 @@ def evaluate(model_fn, labels, mask):
 
 
 def train(model_name, dataset, epochs=20, hidden=None, layers=None, heads=8, lr=1e-2, weight_decay=5e-4,
-          quiet=False):
+          quiet=False, attention="quantized", checkpoint=None):
     """One of the reference's three training drivers (test_gcn.py:183-275, test_gat.py:236-330,
-    test_HGT.py:70-130).  Returns (mean ms per epoch after the first three, final loss)."""
+    test_HGT.py:70-130).  ``attention`` / ``checkpoint``: the HGT layer's (``gat.HGTLayer``); with a checkpoint the
+    read-out keeps its input in 8 bits too.  Returns (mean ms per epoch after the first three, final loss)."""
     g = load_graph_train(dataset)
     feats, labels, train_mask = g.ndata["feat"], g.ndata["label"], g.ndata["train_mask"]
     if model_name == "gcn":
@@ -209,11 +211,13 @@ def train(model_name, dataset, epochs=20, hidden=None, layers=None, heads=8, lr=
         fwd = lambda: model(feats)
     elif model_name == "hgt":
         hidden = hidden or 256
-        model = HGT(feats.size(1), hidden, heads).cuda()
+        model = HGT(feats.size(1), hidden, heads, attention, checkpoint).cuda()
         fwd = lambda: model(g, feats)
     else:
         raise ValueError("model must be gcn, gat or hgt")
-    proj = nn.Linear(hidden, g.n_classes).cuda()  # "proj to predict" (test_gcn.py:229)
+    if model_name != "hgt" and (attention != "quantized" or checkpoint):
+        raise ValueError("attention and checkpoint are options of the hgt model")
+    proj = (CheckpointLinear if checkpoint else nn.Linear)(hidden, g.n_classes).cuda()  # "proj to predict" (test_gcn.py:229)
     opt = torch.optim.Adam(list(model.parameters()) + list(proj.parameters()), lr=lr, weight_decay=weight_decay)
     dur, loss = [], None
     for epoch in range(epochs):
@@ -346,7 +350,14 @@ def main():
     ap.add_argument("--n-label-iters", type=int, default=0, help="arxiv models: refinement passes (needs --use-labels)")
     ap.add_argument("--mask-rate", type=float, default=0.5, help="arxiv models: share of training nodes drawn per epoch")
     ap.add_argument("--edge-drop", type=float, default=0.0, help="arxiv-gat: share of edges dropped per layer and epoch")
+    ap.add_argument("--attention", choices=["quantized", "recompute"], default="quantized",
+                    help="hgt: the int8 operator chain, or one fp32 pass that keeps nothing per edge")
+    ap.add_argument("--checkpoint", choices=["int8"], default=None, help="hgt with --attention recompute: what is kept in 8 bits")
     args = ap.parse_args()
+    if args.model != "hgt" and (args.attention != "quantized" or args.checkpoint):
+        ap.error("--attention and --checkpoint are options of --model hgt")
+    if args.checkpoint and args.attention != "recompute":
+        ap.error("--checkpoint needs --attention recompute")
     if args.model.startswith("linkpred"):
         which = args.model.partition("-")[2] or "gcn"
         ms, loss = train_link_pred(args.dataset, args.epochs, args.n_hidden or (256 if which != "gat" else 64),
@@ -360,7 +371,7 @@ def main():
         ms, loss = train_hetero_hgt(args.epochs, args.n_hidden or 256, min(args.num_heads, 4))
     else:
         ms, loss = train(args.model, args.dataset, args.epochs, args.n_hidden, args.n_layers, args.num_heads, args.lr,
-                         args.weight_decay)
+                         args.weight_decay, attention=args.attention, checkpoint=args.checkpoint)
     print("mean fwd+bwd {:.3f} ms/epoch, final loss {:.4f}".format(ms, loss))
 
 

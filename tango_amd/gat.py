@@ -15,6 +15,7 @@ from .kernels import cuda_kernels, quantize_heads, refuse_capture
 from .SDDMM import sddmm_u_add_v, sddmm_u_dot_v
 from .SPMM import spmm_u_mul_e
 from .edge_softmax import edge_softmax, gat_edge_attention
+from .graph_attention import graph_attention
 
 
 # Whether the GAT layers run u_add_v + LeakyReLU + edge softmax as one op (gat_edge_attention); the separate ops
@@ -173,10 +174,20 @@ class GAT(nn.Module):
 
 class HGTLayer(nn.Module):
     """evaluation/test_HGT.py:27-67, the class the reference calls HGT: one attention layer over a
-    homogenised graph (it has no per-type weights)."""
+    homogenised graph (it has no per-type weights).
 
-    def __init__(self, in_dim, out_dim, n_heads):
+    ``attention="quantized"`` (default) is the reference's chain in int8: dot SDDMM, edge softmax, weighted SpMM, with
+    an [E, heads] tensor between each two.  ``"recompute"`` runs ``graph_attention`` on the projections in fp32
+    instead: one pass, nothing kept per edge, probabilities formed again in the backward pass.  ``checkpoint="int8"``
+    (with "recompute"): queries, keys and values are kept in 8 bits between the passes."""
+
+    def __init__(self, in_dim, out_dim, n_heads, attention="quantized", checkpoint=None):
         super().__init__()
+        if attention not in ("quantized", "recompute"):
+            raise ValueError("HGTLayer: attention must be 'quantized' or 'recompute'")
+        if checkpoint not in (None, "int8") or (checkpoint and attention != "recompute"):
+            raise ValueError("HGTLayer: checkpoint must be None, or 'int8' with attention='recompute'")
+        self.attention, self.checkpoint = attention, checkpoint
         self.out_dim, self.n_heads, self.d_k = out_dim, n_heads, out_dim // n_heads
         self.sqrt_dk = math.sqrt(self.d_k)
         self.q_linear = QLinear(in_dim, out_dim)
@@ -200,9 +211,15 @@ class HGTLayer(nn.Module):
         (k, s_k), (v, s_v), (q, s_q) = shared_input_linears(
             h, (self.k_linear, self.v_linear, self.q_linear), s_h, then=(self.attn_linear, self.msg_linear, None))
         k, v, q = (t.view(-1, self.n_heads, self.d_k) for t in (k, v, q))
+        if self.attention == "recompute":
+            t = graph_attention(g, q, k, v, 1.0 / self.sqrt_dk, checkpoint=self.checkpoint).reshape(-1, self.out_dim)
+            return self._project(t, return_scale)
         t = sddmm_u_dot_v.apply(g, k, q, s_k, s_q, 1.0 / self.sqrt_dk)  # "/ sqrt_dk" folded into the scales
         attn, s_attn = edge_softmax(g, t, want_scale=True)  # the softmax kernel also finds the scale of its output
         t = spmm_u_mul_e.apply(g, v, attn, None, s_v, None, s_attn).reshape(-1, self.out_dim)
+        return self._project(t, return_scale)
+
+    def _project(self, t, return_scale):
         if return_scale:
             return Qlinear_func_reduce.apply(t, self.a_linear.weight, self.a_linear.bias)
         return self.a_linear(t)
@@ -490,10 +507,10 @@ class HGTStack(nn.Module):
     """Several HGT layers back to back with a linear read-out, the shape of the reference's
     driver loop (evaluation/test_HGT.py:87-96: model, then ``proj_layer``)."""
 
-    def __init__(self, in_dim, hidden, n_classes, n_heads, n_layers=2):
+    def __init__(self, in_dim, hidden, n_classes, n_heads, n_layers=2, attention="quantized", checkpoint=None):
         super().__init__()
         dims = [in_dim] + [hidden] * n_layers
-        self.layers = nn.ModuleList(HGTLayer(dims[i], dims[i + 1], n_heads) for i in range(n_layers))
+        self.layers = nn.ModuleList(HGTLayer(dims[i], dims[i + 1], n_heads, attention, checkpoint) for i in range(n_layers))
         self.proj = nn.Linear(hidden, n_classes)
 
     def forward(self, g, h):
