@@ -602,11 +602,11 @@ int tango_batchnorm_bwd_f32(float* dx, float* dgamma, float* dbeta, const float*
    the last run of a row may be shorter, group >= cols gives one run a row.  Per run
      scale = max|x| / 127 (at most the largest whose 127-fold is finite),  q = the integer nearest to 127 x / max|x|, ties to even (decided exactly),
    and q * scale is the value held.  A run with an infinity or a NaN gets scale NaN and q = 0 (every value of it comes
-   back as NaN); a run of zeros gets scale 0.  scale: [rows, ceil(cols / group)], contiguous.  Rows that start on
+   back as NaN); a run of zeros gets scale 0.  The scale of (row, run) is at row * scale_row + run * scale_run.  Rows that start on
    16-byte multiples and runs that are a multiple of 16 bytes take the widest loads; anything else is taken too. */
-int tango_pack_i8(int8_t* q, int64_t ldq, float* scale, const void* x, int dtype, int64_t rows,
-                  int64_t cols, int64_t ldx, int64_t group, tango_stream_t stream);
-/* x[r, c] = q[r, c] * scale[r, c / group] in fp32, then rounded to dtype. */
+int tango_pack_i8(int8_t* q, int64_t ldq, float* scale, int64_t scale_row, int64_t scale_run, const void* x,
+                  int dtype, int64_t rows, int64_t cols, int64_t ldx, int64_t group, tango_stream_t stream);
+/* x[r, c] = q[r, c] * scale[r, c / group] in fp32, then rounded to dtype.  scale: [rows, ceil(cols / group)]. */
 int tango_unpack_i8(void* x, int dtype, int64_t ldx, const int8_t* q, int64_t ldq, const float* scale,
                     int64_t rows, int64_t cols, int64_t group, tango_stream_t stream);
 
@@ -631,7 +631,8 @@ typedef struct tango_attention {
     int checkpoint;                                 /* backward only: q, k, v are int8 with the scales below */
     const void *q, *k, *v;                          /* element (r, h, i) at r * row + h * head + i */
     int64_t q_row, q_head, k_row, k_head, v_row, v_head;
-    const float *q_scale, *k_scale, *v_scale;       /* [rows, heads of the tensor]: a tango_pack_i8 with group = dim */
+    const float *q_scale, *k_scale, *v_scale;       /* of (row r, head h) at r * .._row + h * .._head (k, v: kv_..) */
+    int64_t q_scale_row, q_scale_head, kv_scale_row, kv_scale_head;
     float scale;
 } tango_attention;
 
@@ -645,9 +646,9 @@ typedef struct tango_attn_items {
     const int32_t* edge_ids; /* [num_edges] or NULL (a slot's number is its edge's id): what edge_mask is indexed by */
 } tango_attn_items;
 
-/* Bytes of scratch for the forward pass (by_src NULL) or the backward pass. */
+/* Bytes of scratch for the forward pass (by_src NULL) or the backward pass; masked: a call with an edge_mask. */
 size_t tango_graph_attention_workspace(const tango_attention* t, const tango_attn_items* by_dst,
-                                       const tango_attn_items* by_src);
+                                       const tango_attn_items* by_src, int masked);
 /* out [num_dst, heads, dim] contiguous.  edge_mask: [num_edges] bytes by edge id, 0 = the edge takes no part (whatever
    its key and value hold); NULL: all do.  With checkpoint set: TANGO_ERR_UNSUPPORTED. */
 int tango_graph_attention_fwd(void* out, const tango_attention* t, const tango_attn_items* by_dst,

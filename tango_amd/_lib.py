@@ -77,11 +77,11 @@ SIGNATURES = {
     "tango_edge_softmax_fwd_ex": (I, [P, P, P, P, P, P, P, P, P, P, P, P, I64, I64, I64, F, P, SZ, P]),
     "tango_edge_softmax_bwd_ex": (I, [P, P, P, P, P, P, P, P, I64, I64, I64, F, P, SZ, P]),
     "tango_edge_softmax_bwd": (I, [P, P, P, P, P, P, I64, I64, I64, F, P, SZ, P]),
-    "tango_pack_i8": (I, [P, I64, P, P, I, I64, I64, I64, I64, P]),
+    "tango_pack_i8": (I, [P, I64, P, I64, I64, P, I, I64, I64, I64, I64, P]),
     "tango_unpack_i8": (I, [P, I, I64, P, I64, P, I64, I64, I64, P]),
     "tango_weight_grad_i8_workspace": (SZ, [I64, I64, I64, I64]),
     "tango_weight_grad_i8": (I, [P, P, P, I, I64, P, I64, P, I64, I64, I64, I64, P, SZ, P]),
-    "tango_graph_attention_workspace": (SZ, [P, P, P]),
+    "tango_graph_attention_workspace": (SZ, [P, P, P, I]),
     "tango_graph_attention_fwd": (I, [P, P, P, P, P, SZ, P]),
     "tango_graph_attention_bwd": (I, [P, P, P, P, P, I64, I64, P, P, P, P, SZ, P]),
 }
@@ -102,7 +102,8 @@ class Attention(C.Structure):
     _fields_ = [(n, I64) for n in ("num_dst", "num_src", "heads", "kv_heads", "dim")] + \
                [("dtype", I), ("checkpoint", I)] + [(n, P) for n in ("q", "k", "v")] + \
                [(n, I64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")] + \
-               [(n, P) for n in ("q_scale", "k_scale", "v_scale")] + [("scale", F)]
+               [(n, P) for n in ("q_scale", "k_scale", "v_scale")] + \
+               [(n, I64) for n in ("q_scale_row", "q_scale_head", "kv_scale_row", "kv_scale_head")] + [("scale", F)]
 
 
 class AttnItems(C.Structure):

@@ -67,6 +67,16 @@ def _rows_of(x):
     return x.reshape(rows, cols)
 
 
+def pack_rows(x, group, scale):
+    """The int8 values of a 2-D tensor with contiguous columns; its scales go into ``scale`` [rows, runs], any strides."""
+    rows, cols = x.shape
+    ld = (cols + 15) // 16 * 16
+    values = torch.empty((rows, ld), dtype=torch.int8, device=x.device)[:, :cols]
+    check(_L.tango_pack_i8(_ptr(values), ld, _ptr(scale), scale.stride(0), scale.stride(1), _ptr(x), DTYPES[x.dtype], rows, cols,
+                           x.stride(0) if rows > 1 else cols, group, _stream()), "pack")
+    return values
+
+
 def pack(x, group=None):
     """The 8-bit form of ``x`` [..., cols] (fp32, bf16 or fp16 on the GPU): per run of ``group`` consecutive columns
     (None: the whole row; the last run of a row may be shorter) the scale max|x| / 127 and the integers nearest to
@@ -82,12 +92,8 @@ def pack(x, group=None):
     group = int(group)
     with on_device_of(x):
         flat = _rows_of(x.detach())
-        rows = flat.size(0)
-        ld = (cols + 15) // 16 * 16
-        values = torch.empty((rows, ld), dtype=torch.int8, device=x.device)[:, :cols]
-        scale = torch.empty((rows, -(-cols // group)), dtype=torch.float32, device=x.device)
-        check(_L.tango_pack_i8(_ptr(values), ld, _ptr(scale), _ptr(flat), DTYPES[x.dtype], rows, cols,
-                               flat.stride(0) if rows > 1 else cols, group, _stream()), "pack")
+        scale = torch.empty((flat.size(0), -(-cols // group)), dtype=torch.float32, device=x.device)
+        values = pack_rows(flat, group, scale)
     return Packed(values, scale, group, x.shape, x.dtype)
 
 

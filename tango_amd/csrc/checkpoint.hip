@@ -18,7 +18,7 @@ struct PackArgs {
     const void* x;
     int8_t* q;
     float* scale;
-    int64_t rows, ldx, ldq;
+    int64_t rows, ldx, ldq, scale_row, scale_run;
     uint32_t total;  // runs of this launch: rows * groups
     int cols, group, lanes;  // lanes: a power of two, one run each lane group
     FastDiv groups;
@@ -97,13 +97,15 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
         uint32_t top[UN];
         int64_t row[UN];
         int col[UN], len[UN];
+        uint32_t run[UN];
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
             const uint32_t id = first + u * stride;
             const bool ok = id < a.total;
             const uint32_t rw = a.groups.div(ok ? id : 0);
             row[u] = rw;
-            col[u] = static_cast<int>((ok ? id : 0) - rw * a.groups.d) * a.group;
+            run[u] = (ok ? id : 0) - rw * a.groups.d;
+            col[u] = static_cast<int>(run[u]) * a.group;
             len[u] = ok ? (a.cols - col[u] < a.group ? a.cols - col[u] : a.group) : 0;
             const T* src = static_cast<const T*>(a.x) + row[u] * a.ldx + col[u];
 #pragma unroll
@@ -143,7 +145,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
                 }
                 o.store(dst + c);
             }
-            if (lane == 0) a.scale[first + u * stride] = r.scale;
+            if (lane == 0) a.scale[row[u] * a.scale_row + run[u] * a.scale_run] = r.scale;
         }
     }
 }
@@ -173,7 +175,7 @@ __global__ __launch_bounds__(256) void pack_long_kernel(const PackArgs a) {
         int8_t* dst = a.q + row * a.ldq + col;
         for (int c = threadIdx.x; c < len; c += 256)
             dst[c] = static_cast<int8_t>(t >= 0x7f800000u ? 0 : run_quant(widen(src[c]), r));
-        if (threadIdx.x == 0) a.scale[id] = r.scale;
+        if (threadIdx.x == 0) a.scale[row * a.scale_row + (id - rw * a.groups.d) * a.scale_run] = r.scale;
     }
 }
 
@@ -297,11 +299,12 @@ using namespace tango;
 
 extern "C" {
 
-int tango_pack_i8(int8_t* q, int64_t ldq, float* scale, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
-                  int64_t group, tango_stream_t stream) {
+int tango_pack_i8(int8_t* q, int64_t ldq, float* scale, int64_t scale_row, int64_t scale_run, const void* x, int dtype,
+                  int64_t rows, int64_t cols, int64_t ldx, int64_t group, tango_stream_t stream) {
     const int rc = check_pack(x, dtype, rows, cols, ldx, group, q, ldq, scale);
     if (rc != TANGO_OK || rows == 0 || cols == 0) return rc;
     if (rows > 1 && ldq < cols) return TANGO_ERR_INVALID_ARG;  // rows of the result would overlap
+    if (scale_row < 0 || scale_run < 0) return TANGO_ERR_INVALID_ARG;
     if (group > cols) group = cols;
     const int64_t groups = ceil_div(cols, group);
     const int vec = piece_of(x, dtype, cols, ldx, group, q, ldq);
@@ -311,7 +314,9 @@ int tango_pack_i8(int8_t* q, int64_t ldq, float* scale, const void* x, int dtype
         a.rows = rows - r0 < slab ? rows - r0 : slab;
         a.x = static_cast<const char*>(x) + r0 * ldx * element_size(dtype);
         a.q = q + r0 * ldq;
-        a.scale = scale + r0 * groups;
+        a.scale = scale + r0 * scale_row;
+        a.scale_row = scale_row;
+        a.scale_run = scale_run;
         a.ldx = ldx;
         a.ldq = ldq;
         a.total = static_cast<uint32_t>(a.rows * groups);

@@ -18,6 +18,35 @@ struct Pack {
 #pragma unroll
         for (int i = 0; i < kWords; ++i) w[i] = 0;
     }
+    // p at any multiple of an element: global memory takes vector accesses at any address
+    __device__ __forceinline__ void load_any(const T* p) {
+        static_assert(kBytes == 8 || kBytes % 16 == 0, "whole vectors");
+        if constexpr (kBytes == 8) {
+            typedef u32x2 U __attribute__((aligned(1)));
+            const u32x2 t = *reinterpret_cast<const U*>(p);
+            w[0] = t[0];
+            w[1] = t[1];
+        } else {
+            typedef u32x4 U __attribute__((aligned(1)));
+#pragma unroll
+            for (int i = 0; i < kBytes / 16; ++i) {
+                const u32x4 t = reinterpret_cast<const U*>(p)[i];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[4 * i + j] = t[j];
+            }
+        }
+    }
+    __device__ __forceinline__ void store_any(T* p) const {
+        static_assert(kBytes % 16 == 0, "whole vectors");
+        typedef u32x4 U __attribute__((aligned(1)));
+#pragma unroll
+        for (int i = 0; i < kBytes / 16; ++i) {
+            u32x4 t;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = w[4 * i + j];
+            reinterpret_cast<U*>(p)[i] = t;
+        }
+    }
     // p aligned to min(kBytes, 16)
     __device__ __forceinline__ void load(const T* p) {
         if constexpr (kBytes >= 16) {

@@ -44,10 +44,32 @@ static int check_items(const tango_attn_items* i, int64_t rows) {
 
 static int64_t align256(int64_t b) { return (b + 255) & ~255LL; }
 
+static int64_t masked_bytes(const tango_attn_items& i) { return align256(i.num_edges * 4); }
 static int64_t forward_part_bytes(const tango_attention& t, const tango_attn_items& i) {
     return align256(i.num_parts * t.heads * (t.dim + 2) * 4);
 }
-static int64_t stats_bytes(const tango_attention& t) { return align256(t.num_dst * t.heads * 8); }
+// Whether the rows that a pass gathers from are more than the eight L2s of 4 MB hold.
+static bool far_rows(int64_t rows, int64_t row_bytes) { return rows * row_bytes > (32LL << 20); }
+
+static int64_t held_size(const tango_attention& t) { return t.checkpoint ? 1 : element_size(t.dtype); }
+
+static bool keys_far(const tango_attention& t) { return far_rows(t.num_src, 2 * t.kv_heads * t.dim * held_size(t)); }
+static bool queries_far(const tango_attention& t) {
+    return far_rows(t.num_dst, t.heads * t.dim * (held_size(t) + element_size(t.dtype)));
+}
+
+static int query_tile_log(const tango_attention& t) {
+    return head_tile_log(static_cast<int>(t.heads), static_cast<int>(t.heads / t.kv_heads), static_cast<int>(t.dim), held_size(t), 256);
+}
+static int key_tile_log(const tango_attention& t) {
+    return head_tile_log(static_cast<int>(t.kv_heads), 1, static_cast<int>(t.dim), held_size(t), queries_far(t) ? 512 : 256);
+}
+
+// Query heads of a tile of the dk, dv pass; the statistics of the last tile are padded to as many.
+static int stats_heads(const tango_attention& t) { return static_cast<int>(t.heads / t.kv_heads) << key_tile_log(t); }
+static int64_t stats_bytes(const tango_attention& t) {
+    return align256(ceil_div(t.heads, stats_heads(t)) * stats_heads(t) * t.num_dst * (t.checkpoint ? 16 : 8));
+}
 static int64_t backward_part_bytes(const tango_attention& t, const tango_attn_items& d, const tango_attn_items& s) {
     const int64_t a = align256(d.num_parts * t.heads * (2 * t.dim + 3) * 4), b = align256(s.num_parts * t.kv_heads * 2 * t.dim * 4);
     return a > b ? a : b;
@@ -56,7 +78,7 @@ static int64_t backward_part_bytes(const tango_attention& t, const tango_attn_it
 static int check_operands(const tango_attention& t) {
     if ((t.num_dst && !t.q) || (t.num_src && (!t.k || !t.v))) return TANGO_ERR_INVALID_ARG;
     if (t.checkpoint && ((t.num_dst && !t.q_scale) || (t.num_src && (!t.k_scale || !t.v_scale)))) return TANGO_ERR_INVALID_ARG;
-    const int64_t size = t.checkpoint ? 1 : element_size(t.dtype);
+    const int64_t size = held_size(t);
     if (!aligned_to(t.q, size) || !aligned_to(t.k, size) || !aligned_to(t.v, size)) return TANGO_ERR_INVALID_ARG;
     return TANGO_OK;
 }
@@ -86,23 +108,37 @@ static void fill_args(AttnArgs& a, const tango_attention& t) {
     a.rep = a.heads / a.kv_heads;
     a.dim = static_cast<int>(t.dim);
     a.scale = t.scale;
+    a.num_dst = t.num_dst;
+    a.qs_row = t.q_scale_row;
+    a.qs_head = t.q_scale_head;
+    a.kvs_row = t.kv_scale_row;
+    a.kvs_head = t.kv_scale_head;
+    a.stats_heads = stats_heads(t);
 }
 
-static void use_items(AttnArgs& a, JoinArgs& j, const tango_attn_items& i, const uint8_t* mask, int heads) {
+static void use_items(AttnArgs& a, JoinArgs& j, const tango_attn_items& i, const uint8_t* mask, int32_t* masked, int tile_log, bool far,
+                      hipStream_t s) {
     a.items = reinterpret_cast<const int4*>(i.items);
     a.num_items = i.num_items;
     a.indices = i.indices;
-    a.edge_ids = i.edge_ids;
-    a.mask = mask;
+    if (mask && i.num_edges) {
+        hipLaunchKernelGGL(attn_mask_kernel, dim3(grid_for(i.num_edges, 256)), dim3(256), 0, s, masked, i.indices, i.edge_ids, mask,
+                           static_cast<uint32_t>(i.num_edges));
+        a.indices = masked;
+    }
+    a.tile_log = tile_log;
+    a.tile_slow = far;
     j.split = reinterpret_cast<const int4*>(i.split);
     j.parts = a.parts;
     j.out = a.out;
     j.out2 = a.out2;
     j.stats = a.stats;
-    j.heads = heads;
+    j.q_scale = a.q_scale;
+    j.num_dst = a.num_dst;
+    j.qs_row = a.qs_row;
+    j.qs_head = a.qs_head;
+    j.stats_heads = a.stats_heads;
     j.dim = a.dim;
-    j.width = 1;
-    while (j.width < a.dim) j.width <<= 1;
     j.scale = a.scale;
 }
 
@@ -112,10 +148,12 @@ using namespace tango;
 
 extern "C" {
 
-size_t tango_graph_attention_workspace(const tango_attention* t, const tango_attn_items* by_dst, const tango_attn_items* by_src) {
+size_t tango_graph_attention_workspace(const tango_attention* t, const tango_attn_items* by_dst, const tango_attn_items* by_src,
+                                       int masked) {
     if (check_shape(t) != TANGO_OK || !by_dst) return 0;
-    if (!by_src) return static_cast<size_t>(forward_part_bytes(*t, *by_dst));
-    return static_cast<size_t>(stats_bytes(*t) + backward_part_bytes(*t, *by_dst, *by_src));
+    const int64_t mask = masked ? masked_bytes(*by_dst) : 0;
+    if (!by_src) return static_cast<size_t>(mask + forward_part_bytes(*t, *by_dst));
+    return static_cast<size_t>(mask + stats_bytes(*t) + backward_part_bytes(*t, *by_dst, *by_src));
 }
 
 int tango_graph_attention_fwd(void* out, const tango_attention* t, const tango_attn_items* by_dst, const uint8_t* edge_mask,
@@ -127,15 +165,17 @@ int tango_graph_attention_fwd(void* out, const tango_attention* t, const tango_a
     if (t->checkpoint) return TANGO_ERR_UNSUPPORTED;  // the forward pass runs on the tensors themselves
     if (t->num_dst == 0) return TANGO_OK;
     if (!out || (by_dst->num_edges && t->num_src == 0)) return TANGO_ERR_INVALID_ARG;
-    const int64_t need = forward_part_bytes(*t, *by_dst);
+    const int64_t mask_bytes = edge_mask ? masked_bytes(*by_dst) : 0;
+    const int64_t need = mask_bytes + forward_part_bytes(*t, *by_dst);
     if (need && (!workspace || static_cast<int64_t>(workspace_bytes) < need || !aligned_to(workspace, 16))) return TANGO_ERR_WORKSPACE;
     AttnArgs a;
     JoinArgs j = JoinArgs();
     fill_args(a, *t);
     a.out = out;
-    a.parts = static_cast<float*>(workspace);
-    use_items(a, j, *by_dst, edge_mask, a.heads);
-    const int64_t size = element_size(t->dtype), vec = size == 4 ? 4 : 8;
+    int32_t* masked = static_cast<int32_t*>(workspace);
+    a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + mask_bytes);
+    const int64_t size = element_size(t->dtype), vec = attention_vec(size);
+    use_items(a, j, *by_dst, edge_mask, masked, query_tile_log(*t), keys_far(*t), as_stream(stream));
     const bool aligned = t->dim % vec == 0 && rows_aligned(t->q, t->q_row, t->q_head, vec, size) &&
                          rows_aligned(t->k, t->k_row, t->k_head, vec, size) && rows_aligned(t->v, t->v_row, t->v_head, vec, size) &&
                          aligned_to(out, 16);
@@ -154,9 +194,10 @@ int tango_graph_attention_bwd(void* dq, void* dk, void* dv, const tango_attentio
     if (by_dst->num_edges != by_src->num_edges || (t->num_dst && !dout)) return TANGO_ERR_INVALID_ARG;
     if (by_dst->num_edges && (t->num_src == 0 || t->num_dst == 0)) return TANGO_ERR_INVALID_ARG;
     if (!dq && !dk && !dv) return TANGO_OK;
-    const int64_t need = stats_bytes(*t) + backward_part_bytes(*t, *by_dst, *by_src);
+    const int64_t mask_bytes = edge_mask ? masked_bytes(*by_dst) : 0;
+    const int64_t need = mask_bytes + stats_bytes(*t) + backward_part_bytes(*t, *by_dst, *by_src);
     if (need && (!workspace || static_cast<int64_t>(workspace_bytes) < need || !aligned_to(workspace, 16))) return TANGO_ERR_WORKSPACE;
-    const int64_t size = t->checkpoint ? 1 : element_size(t->dtype), vec = size == 4 ? 4 : 8;
+    const int64_t size = t->checkpoint ? 1 : element_size(t->dtype), vec = attention_vec(size);
     const int64_t gsize = element_size(t->dtype);
     const bool aligned = t->dim % vec == 0 && rows_aligned(t->q, t->q_row, t->q_head, vec, size) &&
                          rows_aligned(t->k, t->k_row, t->k_head, vec, size) && rows_aligned(t->v, t->v_row, t->v_head, vec, size) &&
@@ -168,11 +209,12 @@ int tango_graph_attention_bwd(void* dq, void* dk, void* dv, const tango_attentio
     a.dout = dout;
     a.do_row = dout_row;
     a.do_head = dout_head;
-    a.stats = static_cast<float2*>(workspace);
-    a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(*t));
+    int32_t* masked = static_cast<int32_t*>(workspace);
+    a.stats = reinterpret_cast<float*>(static_cast<char*>(workspace) + mask_bytes);
+    a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + mask_bytes + stats_bytes(*t));
     if (t->num_dst) {
         a.out = dq;
-        use_items(a, j, *by_dst, edge_mask, a.heads);
+        use_items(a, j, *by_dst, edge_mask, masked, query_tile_log(*t), keys_far(*t), as_stream(stream));
         if (!launch_any(*t, kPassQuery, a, j, by_dst->num_split, aligned, as_stream(stream))) return TANGO_ERR_UNSUPPORTED;
         rc = launch_status();
         if (rc != TANGO_OK) return rc;
@@ -180,7 +222,7 @@ int tango_graph_attention_bwd(void* dq, void* dk, void* dv, const tango_attentio
     if (t->num_src && (dk || dv)) {
         a.out = dk;
         a.out2 = dv;
-        use_items(a, j, *by_src, edge_mask, a.kv_heads);
+        use_items(a, j, *by_src, edge_mask, masked, key_tile_log(*t), queries_far(*t), as_stream(stream));
         if (!launch_any(*t, kPassKeyValue, a, j, by_src->num_split, aligned, as_stream(stream))) return TANGO_ERR_UNSUPPORTED;
         rc = launch_status();
     }

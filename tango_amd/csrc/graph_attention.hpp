@@ -19,9 +19,18 @@
 // in item order: nothing here depends on scheduling, and there are no atomics.
 //
 // Lanes.  An item and a tile of heads belong to G lanes: LPH lanes for each head, VEC elements (16 bytes of the
-// gathered type) each, and as many neighbouring heads as bring the gathered piece of a row to 128 bytes, the line
-// of L2.  The head tile varies fastest over the workgroups: consecutive workgroups go to different XCDs, so an L2
-// sees the key and value columns of few heads (with eight tiles: of one).
+// gathered type) each, and as many neighbouring heads as bring the gathered piece of a row to 256 bytes, two lines of L2
+// (fp32 [169343, 8, 32] with 1.3 M edges: forward 390 us, 395 us with 128 bytes, 404 us with 512).  The dk, dv pass takes
+// 512 bytes unless all it gathers from fits the L2s: a line of statistics goes with each piece of a row (at
+// [232965, 8, 32] bf16 and 9.4 M edges 1440 us, 1570 us with 256 bytes, 1740 us with 128; at 19717 rows and 0.2 M edges
+// 31 us against 28 us with 256).
+//
+// What bounds the passes: two gathered rows an edge, most of them from beyond L2 (no graph order is assumed); the
+// fabric behind the L2s delivers 7 to 8 TB/s.  Order of the workgroups: if the rows that a pass gathers from are more
+// than the L2s hold together, the head tile varies slowest, so that all XCDs gather from the same columns and these
+// stay in the 256 MB cache in front of the memory (forward at 169343 rows of 8 x 32 fp32: 390 us against 415 us); if
+// they fit, it varies fastest, so that an XCD's L2 sees the columns of its own tiles only (19717 rows of 8 x 32 bf16:
+// 25 us against 31 us).
 #pragma once
 #include "element.hpp"
 
@@ -31,17 +40,19 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnArgs {
     const void *q, *k, *v, *dout;
-    const float *q_scale, *k_scale, *v_scale;  // int8 operands: one scale per (row, head)
+    const float *q_scale, *k_scale, *v_scale;  // int8 operands: one scale per (row, head), at row * .._row + head * .._head
+    int64_t qs_row, qs_head, kvs_row, kvs_head;
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;  // strides in elements
     void *out, *out2;  // [rows, heads, dim] contiguous
-    float2* stats;     // [destinations, heads]: log2 of the softmax's denominator, delta
+    float* stats;      // per tile of the dk, dv pass [destinations, query heads of the tile]: an AttnStat
+    int64_t num_dst;
+    int stats_heads;   // query heads of such a tile
     float* parts;      // partial results of rows of several items
     const int4* items; // row, first slot, last slot + 1, part or -1
-    const int32_t* indices;
-    const int32_t* edge_ids;  // NULL: a slot's number is its edge's
-    const uint8_t* mask;      // by edge id; NULL: every edge takes part
+    const int32_t* indices;  // the other endpoint of a slot's edge; negative: the edge takes no part
     int64_t num_items;
     int heads, kv_heads, rep, dim, tiles, tile_log;
+    int tile_slow;  // the head tile varies slowest over the workgroups, not fastest
     float scale;
 };
 
@@ -68,59 +79,86 @@ __device__ __forceinline__ float lanes_sum(float x) {
     return x;
 }
 
-// A lane's VEC elements of one head's row.  AL: consecutive elements in vector loads (VEC divides dim and every row
-// start is aligned); else elements lane, lane + LPH, ... one load each.
-template <typename T, int VEC, int LPH, bool AL>
+// How a lane reaches its VEC elements of a head's row (the lanes of a head are numbered j = 0 .. LPH - 1).
+//   kWhole    dim is a multiple of VEC and every row starts on a vector: elements j VEC .. j VEC + VEC - 1.
+//   kShifted  any dim >= VEC, any alignment: the same, except that the last lane with elements is moved back to end with
+//             the row, so that every load is one whole vector inside the row.  What it then shares with its neighbour
+//             is masked to zero.  (dim 250 in fp16: 600 us a pass at [169343, 3, 250] and 1.3 M edges instead of 1800 us
+//             with a load per element.)
+//   kSingle   dim < VEC: one lane, a load per element.
+enum RowMode { kWhole, kShifted, kSingle };
+
+template <int VEC, int LPH, int MODE>
+struct RowLane {
+    int start, first, dim;  // first element held; the first of them that is this lane's (VEC: none)
+    __device__ __forceinline__ RowLane(int j, int d) : dim(d) {
+        if constexpr (MODE == kWhole) {
+            start = j * VEC;
+            first = start < d ? 0 : VEC;
+        } else if constexpr (MODE == kShifted) {
+            start = j * VEC < d - VEC ? j * VEC : d - VEC;
+            first = j * VEC < d ? j * VEC - start : VEC;
+        } else {
+            start = first = 0;
+        }
+    }
+    __device__ __forceinline__ bool mine(int i) const { return MODE == kSingle ? i < dim : i >= first; }
+};
+
+template <typename T, int VEC, int LPH, int MODE>
 struct HeadRow {
     Pack<T, VEC> p;
     __device__ __forceinline__ void zero() { p.zero(); }
-    __device__ __forceinline__ void load(const T* head, int j, int dim) {
-        if constexpr (AL) {
-            if (j * VEC < dim) p.load(head + j * VEC);
-        } else {
-            constexpr int kBits = 8 * static_cast<int>(sizeof(T));
+    // the words are zero before
+    __device__ __forceinline__ void load(const T* head, const RowLane<VEC, LPH, MODE>& lane) {
+        constexpr int kBits = 8 * static_cast<int>(sizeof(T));
+        if constexpr (MODE == kWhole) {
+            if (lane.first == 0) p.load(head + lane.start);
+        } else if constexpr (MODE == kShifted) {
+            p.load_any(head + lane.start);
+            const int cut = lane.first * kBits;  // bits from the front on that are the neighbour's
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int c = i * LPH + j;
-                if (c < dim) {
-                    Pack<T, 1> one;
-                    one.load(head + c);
-                    p.w[i * kBits / 32] |= one.w[0] << (i * kBits % 32);  // the words are zero before
-                }
+            for (int i = 0; i < Pack<T, VEC>::kWords; ++i) {
+                const int c = cut - 32 * i;
+                p.w[i] &= c <= 0 ? 0xffffffffu : c >= 32 ? 0u : 0xffffffffu << (c & 31);
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (i < lane.dim) {
+                    Pack<T, 1> one;
+                    one.load(head + i);
+                    p.w[i * kBits / 32] |= one.w[0] << (i * kBits % 32);
+                }
         }
     }
     __device__ __forceinline__ float get(int i) const { return p.get(i); }
 };
 
-template <typename T, int VEC, int LPH, bool AL>
-__device__ __forceinline__ void store_head(T* head, int j, int dim, const float* v) {
-    if constexpr (AL) {
-        if (j * VEC < dim) {
-            Pack<T, VEC> o;
-            o.set_all(v);
-            o.store(head + j * VEC);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int c = i * LPH + j;
-            if (c < dim) {
-                Pack<T, 1> o;
-                o.set_all(v + i);
-                o.store(head + c);
-            }
-        }
+template <typename T, int VEC, int LPH, int MODE>
+__device__ __forceinline__ void store_head(T* head, const RowLane<VEC, LPH, MODE>& lane, const float* v) {
+    if (MODE != kSingle && lane.first == 0) {
+        Pack<T, VEC> o;
+        o.set_all(v);
+        if constexpr (MODE == kWhole) o.store(head + lane.start);
+        if constexpr (MODE == kShifted) o.store_any(head + lane.start);
+        return;
     }
+    if (MODE == kWhole) return;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+        if (lane.mine(i)) {
+            Pack<T, 1> o;
+            o.set_all(v + i);
+            o.store(head + lane.start + i);
+        }
 }
 
-template <int VEC, int LPH, bool AL>
-__device__ __forceinline__ void store_part(float* head, int j, int dim, const float* v) {
+template <int VEC, int LPH, int MODE>
+__device__ __forceinline__ void store_part(float* head, const RowLane<VEC, LPH, MODE>& lane, const float* v) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        const int c = AL ? j * VEC + i : i * LPH + j;
-        if (c < dim) head[c] = v[i];
-    }
+    for (int i = 0; i < VEC; ++i)
+        if (lane.mine(i)) head[lane.start + i] = v[i];
 }
 
 struct ItemLane {
@@ -134,8 +172,10 @@ __device__ __forceinline__ ItemLane item_lane(const AttnArgs& a, int heads) {
     ItemLane r;
     const int g_log = a.tile_log + __builtin_ctz(LPH);
     const int gl = threadIdx.x & ((1 << g_log) - 1);
-    const int64_t block = blockIdx.x / static_cast<uint32_t>(a.tiles);
-    const int tile = static_cast<int>(blockIdx.x - static_cast<uint32_t>(block) * a.tiles);
+    const uint32_t inner = a.tile_slow ? gridDim.x / static_cast<uint32_t>(a.tiles) : static_cast<uint32_t>(a.tiles);
+    const uint32_t outer_id = blockIdx.x / inner, inner_id = blockIdx.x - outer_id * inner;
+    const int64_t block = a.tile_slow ? inner_id : outer_id;
+    const int tile = static_cast<int>(a.tile_slow ? outer_id : inner_id);
     const int64_t id = block * (256 >> g_log) + (threadIdx.x >> g_log);
     r.head = (tile << a.tile_log) + gl / LPH;
     r.j = gl & (LPH - 1);
@@ -152,18 +192,11 @@ struct Slots {
     bool ok[U];
     __device__ __forceinline__ void load(const AttnArgs& a, int e, int end) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            ok[u] = e + u < end;
-            id[u] = a.indices[ok[u] ? e + u : end - 1];
-        }
-        if (a.mask) {
+        for (int u = 0; u < U; ++u) id[u] = a.indices[e + u < end ? e + u : end - 1];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int slot = ok[u] ? e + u : end - 1;
-                ok[u] = ok[u] && a.mask[a.edge_ids ? a.edge_ids[slot] : slot];
-            }
-        }
+        for (int u = 0; u < U; ++u) ok[u] = e + u < end;
     }
+    __device__ __forceinline__ bool take(int u) const { return ok[u] && id[u] >= 0; }
 };
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -179,19 +212,20 @@ __device__ __forceinline__ float log2_total(float m, float l) { return l == 0.0f
 
 constexpr int kEdgesInFlight = 4;
 
-template <typename T, int VEC, int LPH, bool AL>
+template <typename T, int VEC, int LPH, int MODE>
 __global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnArgs a) {
     constexpr int U = kEdgesInFlight;
     const ItemLane L = item_lane<LPH>(a, a.heads);
     if (!L.on) return;
+    const RowLane<VEC, LPH, MODE> lane(L.j, a.dim);
     const int kvh = L.head / a.rep;
     const T* k = static_cast<const T*>(a.k) + kvh * a.k_head;
     const T* v = static_cast<const T*>(a.v) + kvh * a.v_head;
     float q[VEC], acc[VEC];
     {
-        HeadRow<T, VEC, LPH, AL> r;
+        HeadRow<T, VEC, LPH, MODE> r;
         r.zero();
-        r.load(static_cast<const T*>(a.q) + L.it.x * a.q_row + L.head * a.q_head, L.j, a.dim);
+        r.load(static_cast<const T*>(a.q) + L.it.x * a.q_row + L.head * a.q_head, lane);
         const float f = a.scale * kLog2e;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
@@ -205,16 +239,18 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnArgs a) {
     if (L.it.y < end) next.load(a, L.it.y, end);
     for (int e = L.it.y; e < end; e += U) {
         cur = next;
-        HeadRow<T, VEC, LPH, AL> kr[U], vr[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) cur.ok[u] = cur.take(u);
+        HeadRow<T, VEC, LPH, MODE> kr[U], vr[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             kr[u].zero();
-            if (cur.ok[u]) kr[u].load(k + cur.id[u] * a.k_row, L.j, a.dim);
+            if (cur.ok[u]) kr[u].load(k + cur.id[u] * a.k_row, lane);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             vr[u].zero();
-            if (cur.ok[u]) vr[u].load(v + cur.id[u] * a.v_row, L.j, a.dim);
+            if (cur.ok[u]) vr[u].load(v + cur.id[u] * a.v_row, lane);
         }
         if (e + U < end) next.load(a, e + U, end);
         float s[U];
@@ -247,45 +283,70 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[i] *= r;
         T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(L.it.x) * a.heads + L.head) * a.dim;
-        store_head<T, VEC, LPH, AL>(out, L.j, a.dim, acc);
+        store_head<T, VEC, LPH, MODE>(out, lane, acc);
     } else {
         float* part = a.parts + (static_cast<int64_t>(L.it.w) * a.heads + L.head) * (a.dim + 2);
         if (L.j == 0) {
             part[0] = m;
             part[1] = l;
         }
-        store_part<VEC, LPH, AL>(part + 2, L.j, a.dim, acc);
+        store_part<VEC, LPH, MODE>(part + 2, lane, acc);
     }
 }
 
 template <typename T>
 struct RowScale {
     static constexpr bool kScaled = __is_same(T, int8_t);
-    static __device__ __forceinline__ float get(const float* scale, int64_t row, int heads, int head) {
-        if constexpr (kScaled) return scale[row * heads + head];
+    static __device__ __forceinline__ float get(const float* scale, int64_t row, int64_t row_step, int64_t head) {
+        if constexpr (kScaled) return scale[row * row_step + head];
         return 1.0f;
     }
 };
 
+// What the dk, dv pass needs of a (destination, query head) beside its rows: log2 of the softmax's denominator, delta, and
+// from checkpoints the query's scale.  Laid out so that what a lane group reads of a destination is contiguous: with
+// all heads of a destination together, a tile of one head would fetch a line for 8 bytes of it (at [169343, 8, 32] fp32
+// and 1.3 M edges that pass took 690 us, 610 us with the tile's alone).
+template <bool SCALED>
+struct AttnStat {
+    static constexpr int kFloats = SCALED ? 4 : 2;
+    static __device__ __forceinline__ void store(float* stats, int64_t num_dst, int per_tile, int64_t row, int head, float total,
+                                                 float delta, float scale) {
+        const int tile = head / per_tile;
+        float* p = stats + ((tile * num_dst + row) * per_tile + (head - tile * per_tile)) * kFloats;
+        if constexpr (SCALED)
+            *reinterpret_cast<float4*>(p) = make_float4(total, delta, scale, 0.0f);
+        else
+            *reinterpret_cast<float2*>(p) = make_float2(total, delta);
+    }
+    static __device__ __forceinline__ float4 load(const float* tile, int64_t at) {
+        if constexpr (SCALED) return *reinterpret_cast<const float4*>(tile + at * 4);
+        const float2 t = *reinterpret_cast<const float2*>(tile + at * 2);
+        return make_float4(t.x, t.y, 1.0f, 0.0f);
+    }
+};
+
 // T: what q, k, v are held in (int8_t: checkpoints, with a scale per row and head); TG: dout and the results
-template <typename T, typename TG, int VEC, int LPH, bool AL>
+template <typename T, typename TG, int VEC, int LPH, int MODE>
 __global__ __launch_bounds__(256) void attn_bwd_q_kernel(const AttnArgs a) {
     constexpr int U = kEdgesInFlight;
     typedef RowScale<T> S;
     const ItemLane L = item_lane<LPH>(a, a.heads);
     if (!L.on) return;
+    const RowLane<VEC, LPH, MODE> lane(L.j, a.dim);
     const int kvh = L.head / a.rep;
     const T* k = static_cast<const T*>(a.k) + kvh * a.k_head;
     const T* v = static_cast<const T*>(a.v) + kvh * a.v_head;
+    const float qs = S::get(a.q_scale, L.it.x, a.qs_row, L.head * a.qs_head);
     float q[VEC], g[VEC], A[VEC], B[VEC];
     {
-        HeadRow<T, VEC, LPH, AL> r;
-        HeadRow<TG, VEC, LPH, AL> o;
+        HeadRow<T, VEC, LPH, MODE> r;
+        HeadRow<TG, VEC, LPH, MODE> o;
         r.zero();
         o.zero();
-        r.load(static_cast<const T*>(a.q) + L.it.x * a.q_row + L.head * a.q_head, L.j, a.dim);
-        o.load(static_cast<const TG*>(a.dout) + L.it.x * a.do_row + L.head * a.do_head, L.j, a.dim);
-        const float f = S::get(a.q_scale, L.it.x, a.heads, L.head) * a.scale * kLog2e;
+        r.load(static_cast<const T*>(a.q) + L.it.x * a.q_row + L.head * a.q_head, lane);
+        o.load(static_cast<const TG*>(a.dout) + L.it.x * a.do_row + L.head * a.do_head, lane);
+        const float f = qs * a.scale * kLog2e;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             q[i] = r.get(i) * f;
@@ -299,7 +360,9 @@ __global__ __launch_bounds__(256) void attn_bwd_q_kernel(const AttnArgs a) {
     if (L.it.y < end) next.load(a, L.it.y, end);
     for (int e = L.it.y; e < end; e += U) {
         cur = next;
-        HeadRow<T, VEC, LPH, AL> kr[U], vr[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) cur.ok[u] = cur.take(u);
+        HeadRow<T, VEC, LPH, MODE> kr[U], vr[U];
         float ks[U], vs[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -307,10 +370,10 @@ __global__ __launch_bounds__(256) void attn_bwd_q_kernel(const AttnArgs a) {
             vr[u].zero();
             ks[u] = vs[u] = 1.0f;
             if (cur.ok[u]) {
-                kr[u].load(k + cur.id[u] * a.k_row, L.j, a.dim);
-                vr[u].load(v + cur.id[u] * a.v_row, L.j, a.dim);
-                ks[u] = S::get(a.k_scale, cur.id[u], a.kv_heads, kvh);
-                vs[u] = S::get(a.v_scale, cur.id[u], a.kv_heads, kvh);
+                kr[u].load(k + cur.id[u] * a.k_row, lane);
+                vr[u].load(v + cur.id[u] * a.v_row, lane);
+                ks[u] = S::get(a.k_scale, cur.id[u], a.kvs_row, kvh * a.kvs_head);
+                vs[u] = S::get(a.v_scale, cur.id[u], a.kvs_row, kvh * a.kvs_head);
             }
         }
         if (e + U < end) next.load(a, e + U, end);
@@ -365,8 +428,8 @@ __global__ __launch_bounds__(256) void attn_bwd_q_kernel(const AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) A[i] = (A[i] - delta * B[i]) * f;
         const int64_t at = static_cast<int64_t>(L.it.x) * a.heads + L.head;
-        if (a.out) store_head<TG, VEC, LPH, AL>(static_cast<TG*>(a.out) + at * a.dim, L.j, a.dim, A);
-        if (L.j == 0) a.stats[at] = make_float2(log2_total(m, l), delta);
+        if (a.out) store_head<TG, VEC, LPH, MODE>(static_cast<TG*>(a.out) + at * a.dim, lane, A);
+        if (L.j == 0) AttnStat<S::kScaled>::store(a.stats, a.num_dst, a.stats_heads, L.it.x, L.head, log2_total(m, l), delta, qs);
     } else {
         float* part = a.parts + (static_cast<int64_t>(L.it.w) * a.heads + L.head) * (2 * a.dim + 3);
         if (L.j == 0) {
@@ -374,28 +437,31 @@ __global__ __launch_bounds__(256) void attn_bwd_q_kernel(const AttnArgs a) {
             part[1] = l;
             part[2] = dsum;
         }
-        store_part<VEC, LPH, AL>(part + 3, L.j, a.dim, A);
-        store_part<VEC, LPH, AL>(part + 3 + a.dim, L.j, a.dim, B);
+        store_part<VEC, LPH, MODE>(part + 3, lane, A);
+        store_part<VEC, LPH, MODE>(part + 3 + a.dim, lane, B);
     }
 }
 
-template <typename T, typename TG, int VEC, int LPH, bool AL>
+template <typename T, typename TG, int VEC, int LPH, int MODE>
 __global__ __launch_bounds__(256) void attn_bwd_kv_kernel(const AttnArgs a) {
     constexpr int U = kEdgesInFlight;
     typedef RowScale<T> S;
     const ItemLane L = item_lane<LPH>(a, a.kv_heads);
     if (!L.on) return;
+    const RowLane<VEC, LPH, MODE> lane(L.j, a.dim);
     const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(L.head) * a.rep * a.q_head;
     const TG* o = static_cast<const TG*>(a.dout) + static_cast<int64_t>(L.head) * a.rep * a.do_head;
+    const int in_tile = L.head & ((1 << a.tile_log) - 1);
+    const float* stats = a.stats + ((L.head >> a.tile_log) * a.num_dst * a.stats_heads + in_tile * a.rep) * AttnStat<S::kScaled>::kFloats;
     float k[VEC], v[VEC], dk[VEC], dv[VEC];
     {
-        HeadRow<T, VEC, LPH, AL> kr, vr;
+        HeadRow<T, VEC, LPH, MODE> kr, vr;
         kr.zero();
         vr.zero();
-        kr.load(static_cast<const T*>(a.k) + L.it.x * a.k_row + L.head * a.k_head, L.j, a.dim);
-        vr.load(static_cast<const T*>(a.v) + L.it.x * a.v_row + L.head * a.v_head, L.j, a.dim);
-        const float f = S::get(a.k_scale, L.it.x, a.kv_heads, L.head) * a.scale * kLog2e;
-        const float fv = S::get(a.v_scale, L.it.x, a.kv_heads, L.head);
+        kr.load(static_cast<const T*>(a.k) + L.it.x * a.k_row + L.head * a.k_head, lane);
+        vr.load(static_cast<const T*>(a.v) + L.it.x * a.v_row + L.head * a.v_head, lane);
+        const float f = S::get(a.k_scale, L.it.x, a.kvs_row, L.head * a.kvs_head) * a.scale * kLog2e;
+        const float fv = S::get(a.v_scale, L.it.x, a.kvs_row, L.head * a.kvs_head);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             k[i] = kr.get(i) * f;
@@ -408,24 +474,22 @@ __global__ __launch_bounds__(256) void attn_bwd_kv_kernel(const AttnArgs a) {
     if (L.it.y < end) next.load(a, L.it.y, end);
     for (int e = L.it.y; e < end; e += U) {
         cur = next;
+#pragma unroll
+        for (int u = 0; u < U; ++u) cur.ok[u] = cur.take(u);
         if (e + U < end) next.load(a, e + U, end);
         for (int r = 0; r < a.rep; ++r) {
-            HeadRow<T, VEC, LPH, AL> qr[U];
-            HeadRow<TG, VEC, LPH, AL> gr[U];
-            float qs[U];
-            float2 st[U];
+            HeadRow<T, VEC, LPH, MODE> qr[U];
+            HeadRow<TG, VEC, LPH, MODE> gr[U];
+            float4 st[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 qr[u].zero();
                 gr[u].zero();
-                qs[u] = 1.0f;
-                st[u] = make_float2(0.0f, 0.0f);
+                st[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (cur.ok[u]) {
-                    const int h = L.head * a.rep + r;
-                    qr[u].load(q + cur.id[u] * a.q_row + r * a.q_head, L.j, a.dim);
-                    gr[u].load(o + cur.id[u] * a.do_row + r * a.do_head, L.j, a.dim);
-                    qs[u] = S::get(a.q_scale, cur.id[u], a.heads, h);
-                    st[u] = a.stats[static_cast<int64_t>(cur.id[u]) * a.heads + h];
+                    qr[u].load(q + cur.id[u] * a.q_row + r * a.q_head, lane);
+                    gr[u].load(o + cur.id[u] * a.do_row + r * a.do_head, lane);
+                    st[u] = AttnStat<S::kScaled>::load(stats, static_cast<int64_t>(cur.id[u]) * a.stats_heads + r);
                 }
             }
 #pragma unroll
@@ -438,10 +502,10 @@ __global__ __launch_bounds__(256) void attn_bwd_kv_kernel(const AttnArgs a) {
                 }
                 t = lanes_sum<LPH>(t);
                 w = lanes_sum<LPH>(w);
-                if constexpr (S::kScaled) t *= qs[u];
+                if constexpr (S::kScaled) t *= st[u].z;
                 const float p = cur.ok[u] ? exp2_fast(t - st[u].x) : 0.0f;
                 float ds = cur.ok[u] ? p * (w - st[u].y) : 0.0f;
-                if constexpr (S::kScaled) ds *= qs[u];
+                if constexpr (S::kScaled) ds *= st[u].z;
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
                     dk[i] = __builtin_fmaf(ds, qr[u].get(i), dk[i]);
@@ -454,97 +518,108 @@ __global__ __launch_bounds__(256) void attn_bwd_kv_kernel(const AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) dk[i] *= a.scale;
         const int64_t at = (static_cast<int64_t>(L.it.x) * a.kv_heads + L.head) * a.dim;
-        if (a.out) store_head<TG, VEC, LPH, AL>(static_cast<TG*>(a.out) + at, L.j, a.dim, dk);
-        if (a.out2) store_head<TG, VEC, LPH, AL>(static_cast<TG*>(a.out2) + at, L.j, a.dim, dv);
+        if (a.out) store_head<TG, VEC, LPH, MODE>(static_cast<TG*>(a.out) + at, lane, dk);
+        if (a.out2) store_head<TG, VEC, LPH, MODE>(static_cast<TG*>(a.out2) + at, lane, dv);
     } else {
         float* part = a.parts + (static_cast<int64_t>(L.it.w) * a.kv_heads + L.head) * (2 * a.dim);
-        store_part<VEC, LPH, AL>(part, L.j, a.dim, dk);
-        store_part<VEC, LPH, AL>(part + a.dim, L.j, a.dim, dv);
+        store_part<VEC, LPH, MODE>(part, lane, dk);
+        store_part<VEC, LPH, MODE>(part + a.dim, lane, dv);
     }
 }
 
-// One workgroup per (row of several items, head): thread t holds element t % width, slice t / width of the parts.
+// Joins the parts of a row of several items.  A workgroup owns 64 of the row's heads * dim elements, one a lane; each of
+// its four waves takes every fourth part, and the four running results are added in order.
 struct JoinArgs {
     const int4* split;  // row, first part, last part + 1
     const float* parts;
     void *out, *out2;
-    float2* stats;
-    int heads, dim, width;  // width: the power of two that holds dim, at most 256
+    float* stats;
+    const float* q_scale;
+    int64_t num_dst, qs_row, qs_head;
+    int stats_heads, heads, dim, windows;
     float scale;
 };
 
 enum JoinKind { kJoinForward, kJoinQuery, kJoinKeyValue };
 
-__device__ __forceinline__ float block_max(float v, float* red) {
-    v = wave_max(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-}
-
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
-}
-
-template <typename T, int KIND>
+template <typename T, int KIND, bool SCALED>
 __global__ __launch_bounds__(256) void attn_join_kernel(const JoinArgs a) {
-    __shared__ float red[4];
-    __shared__ float one[256], two[256];
-    const int4 sp = a.split[blockIdx.x / a.heads];
-    const int head = blockIdx.x % a.heads;
-    const int n = sp.z - sp.y;
     constexpr int kHead = KIND == kJoinForward ? 2 : KIND == kJoinQuery ? 3 : 0;
-    const int64_t len = (KIND == kJoinForward ? 1 : 2) * a.dim + kHead;
-    const int64_t step = len * a.heads;
-    const float* p = a.parts + (static_cast<int64_t>(sp.y) * a.heads + head) * len;
-    const int d = threadIdx.x & (a.width - 1), slice = threadIdx.x / a.width, slices = 256 / a.width;
-    float m = -INFINITY, l = 0.0f, dsum = 0.0f;
+    __shared__ float sm[4][64], sl[4][64], sd[4][64], sx[4][64], sy[4][64];
+    const uint32_t row_id = blockIdx.x / static_cast<uint32_t>(a.windows);
+    const int4 sp = a.split[row_id];
+    const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
+    const int e = static_cast<int>(blockIdx.x - row_id * a.windows) * 64 + lane;
+    const bool on = e < a.heads * a.dim;
+    const int head = on ? e / a.dim : 0, d = on ? e - head * a.dim : 0;
+    const int len = (KIND == kJoinForward ? 1 : 2) * a.dim + kHead;
+    const int64_t step = static_cast<int64_t>(len) * a.heads;
+    const float* p = a.parts + sp.y * step + static_cast<int64_t>(head) * len;
+    const int n = sp.z - sp.y;
+    float m = -INFINITY, l = 0.0f, dsum = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll 4
+    for (int i = slice; i < n; i += 4) {
+        const float* r = p + i * step;
+        const float px = r[kHead + d], py = KIND == kJoinForward ? 0.0f : r[kHead + a.dim + d];
+        if constexpr (KIND == kJoinKeyValue) {
+            x += px;
+            y += py;
+        } else {
+            const float pm = r[0], m_new = fmaxf(m, pm);
+            const float c = rescale(m, m_new), pc = exp2_fast(pm - shift_of(m_new));
+            m = m_new;
+            l = __builtin_fmaf(r[1], pc, l * c);
+            x = __builtin_fmaf(px, pc, x * c);
+            if constexpr (KIND == kJoinQuery) {
+                dsum = __builtin_fmaf(r[2], pc, dsum * c);
+                y = __builtin_fmaf(py, pc, y * c);
+            }
+        }
+    }
+    sx[slice][lane] = x;
+    if constexpr (KIND != kJoinForward) sy[slice][lane] = y;
     if constexpr (KIND != kJoinKeyValue) {
-        for (int i = threadIdx.x; i < n; i += 256) m = fmaxf(m, p[i * step]);
-        m = block_max(m, red);
-        const float shift = shift_of(m);
-        for (int i = threadIdx.x; i < n; i += 256) {
-            const float c = exp2_fast(p[i * step] - shift);
-            l += p[i * step + 1] * c;
-            if constexpr (KIND == kJoinQuery) dsum += p[i * step + 2] * c;
-        }
-        l = block_sum(l, red);
-        if constexpr (KIND == kJoinQuery) dsum = block_sum(dsum, red);
+        sm[slice][lane] = m;
+        sl[slice][lane] = l;
     }
-    float x = 0.0f, y = 0.0f;
-    if (d < a.dim) {
-        const float shift = shift_of(m);
-        for (int i = slice; i < n; i += slices) {
-            const float* r = p + i * step;
-            const float c = KIND == kJoinKeyValue ? 1.0f : exp2_fast(r[0] - shift);
-            x = __builtin_fmaf(r[kHead + d], c, x);
-            if constexpr (KIND != kJoinForward) y = __builtin_fmaf(r[kHead + a.dim + d], c, y);
-        }
-    }
-    one[threadIdx.x] = x;
-    if constexpr (KIND != kJoinForward) two[threadIdx.x] = y;
+    if constexpr (KIND == kJoinQuery) sd[slice][lane] = dsum;
     __syncthreads();
-    if (slice != 0 || d >= a.dim) return;
-    for (int s = 1; s < slices; ++s) {
-        x += one[s * a.width + d];
-        if constexpr (KIND != kJoinForward) y += two[s * a.width + d];
+    if (slice != 0 || !on) return;
+    if constexpr (KIND != kJoinKeyValue) m = fmaxf(fmaxf(sm[0][lane], sm[1][lane]), fmaxf(sm[2][lane], sm[3][lane]));
+    l = dsum = x = y = 0.0f;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        const float c = KIND == kJoinKeyValue ? 1.0f : exp2_fast(sm[s][lane] - shift_of(m));
+        x = __builtin_fmaf(sx[s][lane], c, x);
+        if constexpr (KIND != kJoinForward) y = __builtin_fmaf(sy[s][lane], c, y);
+        if constexpr (KIND != kJoinKeyValue) l = __builtin_fmaf(sl[s][lane], c, l);
+        if constexpr (KIND == kJoinQuery) dsum = __builtin_fmaf(sd[s][lane], c, dsum);
     }
-    const int64_t at = static_cast<int64_t>(sp.x) * a.heads + head;
+    const int64_t at = (static_cast<int64_t>(sp.x) * a.heads + head) * a.dim + d;
     const float r = l == 0.0f ? 0.0f : 1.0f / l;
     if constexpr (KIND == kJoinForward) {
-        static_cast<T*>(a.out)[at * a.dim + d] = static_cast<T>(x * r);
+        static_cast<T*>(a.out)[at] = static_cast<T>(x * r);
     } else if constexpr (KIND == kJoinQuery) {
         const float delta = dsum * r;
-        if (a.out) static_cast<T*>(a.out)[at * a.dim + d] = static_cast<T>((x - delta * y) * (a.scale * r));
-        if (d == 0) a.stats[at] = make_float2(log2_total(m, l), delta);
+        if (a.out) static_cast<T*>(a.out)[at] = static_cast<T>((x - delta * y) * (a.scale * r));
+        if (d == 0)
+            AttnStat<SCALED>::store(a.stats, a.num_dst, a.stats_heads, sp.x, head, log2_total(m, l), delta,
+                                    SCALED ? a.q_scale[sp.x * a.qs_row + head * a.qs_head] : 1.0f);
     } else {
-        if (a.out) static_cast<T*>(a.out)[at * a.dim + d] = static_cast<T>(x * a.scale);
-        if (a.out2) static_cast<T*>(a.out2)[at * a.dim + d] = static_cast<T>(y);
+        if (a.out) static_cast<T*>(a.out)[at] = static_cast<T>(x * a.scale);
+        if (a.out2) static_cast<T*>(a.out2)[at] = static_cast<T>(y);
+    }
+}
+
+// indices with the edges that a mask leaves out made negative: the passes then read one number a slot, not a chain of
+// three (slot, edge id, mask) in front of every gather (forward at 5.3 M edges, heads 8 over 2,
+// fp32: 1040 us with the chain, 550 us and 45 us for this kernel without)
+static __global__ __launch_bounds__(256) void attn_mask_kernel(int32_t* out, const int32_t* indices, const int32_t* edge_ids,
+                                                               const uint8_t* mask, uint32_t n) {
+    const uint32_t stride = gridDim.x * 256;
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+        const bool kept = mask[edge_ids ? static_cast<uint32_t>(edge_ids[i]) : i];
+        out[i] = kept ? indices[i] : -1;
     }
 }
 
@@ -555,56 +630,80 @@ enum AttnPass { kPassForward, kPassQuery, kPassKeyValue };
 template <typename T, typename TG>
 bool launch_attention(AttnPass pass, AttnArgs a, JoinArgs j, int64_t num_split, bool aligned, hipStream_t s);
 
-template <typename T, typename TG, int VEC, int LPH, bool AL>
+// Lanes of a head: a power of two with a vector of VEC elements each.
+inline int head_lanes_log(int dim, int vec) {
+    int log = 0;
+    while ((vec << log) < dim) ++log;
+    return log;
+}
+
+// Elements per lane: 16 bytes of fp32, bf16, fp16; 8 of int8 (whose gradients are four or two times as wide).
+inline int attention_vec(int64_t size) { return size == 4 ? 4 : 8; }
+
+// Neighbouring heads of a lane group, as a power of two: what brings the gathered piece of a row to `bytes`.  Query heads
+// that share a key head count once: their lanes read the same addresses.
+inline int head_tile_log(int heads, int rep, int dim, int64_t size, int64_t bytes) {
+    const int vec = attention_vec(size), lanes = static_cast<int>(bytes / (vec * size));
+    const int lph_log = head_lanes_log(dim, vec);
+    int log = 0;
+    while ((1 << (lph_log + log)) < lanes * rep && (1 << (lph_log + log)) < kWave && (1 << log) < heads) ++log;
+    return log;
+}
+
+template <typename T, typename TG, int VEC, int LPH, int MODE>
 bool launch_attention_lanes(AttnPass pass, AttnArgs& a, hipStream_t s) {
-    const int heads = pass == kPassKeyValue ? a.kv_heads : a.heads;
-    // 128 bytes of a gathered row: eight lanes of 16 bytes, as far as there are heads
-    a.tile_log = 0;
-    while ((LPH << a.tile_log) < 8 && (1 << a.tile_log) < heads) ++a.tile_log;
-    a.tiles = static_cast<int>(ceil_div(heads, 1 << a.tile_log));
     const int64_t per_block = 256 / (LPH << a.tile_log);
     const int64_t blocks = ceil_div(a.num_items, per_block) * a.tiles;
     if (blocks > 0x7fffffffLL) return false;
     if (blocks == 0) return true;
     const dim3 grid(static_cast<uint32_t>(blocks)), block(256);
     if (pass == kPassForward) {
-        if constexpr (__is_same(T, TG)) hipLaunchKernelGGL((attn_fwd_kernel<T, VEC, LPH, AL>), grid, block, 0, s, a);
+        if constexpr (__is_same(T, TG)) hipLaunchKernelGGL((attn_fwd_kernel<T, VEC, LPH, MODE>), grid, block, 0, s, a);
     } else if (pass == kPassQuery) {
-        hipLaunchKernelGGL((attn_bwd_q_kernel<T, TG, VEC, LPH, AL>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((attn_bwd_q_kernel<T, TG, VEC, LPH, MODE>), grid, block, 0, s, a);
     } else {
-        hipLaunchKernelGGL((attn_bwd_kv_kernel<T, TG, VEC, LPH, AL>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((attn_bwd_kv_kernel<T, TG, VEC, LPH, MODE>), grid, block, 0, s, a);
     }
     return true;
 }
 
-template <typename T, typename TG, int VEC, bool AL>
+template <typename T, typename TG, int VEC, int MODE>
 bool launch_attention_vec(AttnPass pass, AttnArgs& a, hipStream_t s) {
-    const int pieces = (a.dim + VEC - 1) / VEC;
-    if (pieces <= 1) return launch_attention_lanes<T, TG, VEC, 1, AL>(pass, a, s);
-    if (pieces <= 2) return launch_attention_lanes<T, TG, VEC, 2, AL>(pass, a, s);
-    if (pieces <= 4) return launch_attention_lanes<T, TG, VEC, 4, AL>(pass, a, s);
-    if (pieces <= 8) return launch_attention_lanes<T, TG, VEC, 8, AL>(pass, a, s);
-    if (pieces <= 16) return launch_attention_lanes<T, TG, VEC, 16, AL>(pass, a, s);
-    if (pieces <= 32) return launch_attention_lanes<T, TG, VEC, 32, AL>(pass, a, s);
-    if constexpr (VEC == 4) return launch_attention_lanes<T, TG, VEC, 64, AL>(pass, a, s);
+    switch (head_lanes_log(a.dim, VEC)) {
+        case 0: return launch_attention_lanes<T, TG, VEC, 1, MODE>(pass, a, s);
+        case 1: return launch_attention_lanes<T, TG, VEC, 2, MODE>(pass, a, s);
+        case 2: return launch_attention_lanes<T, TG, VEC, 4, MODE>(pass, a, s);
+        case 3: return launch_attention_lanes<T, TG, VEC, 8, MODE>(pass, a, s);
+        case 4: return launch_attention_lanes<T, TG, VEC, 16, MODE>(pass, a, s);
+        case 5: return launch_attention_lanes<T, TG, VEC, 32, MODE>(pass, a, s);
+        case 6:
+            if constexpr (VEC == 4) return launch_attention_lanes<T, TG, VEC, 64, MODE>(pass, a, s);
+    }
     return false;
 }
 
 template <typename T, typename TG>
 bool launch_attention(AttnPass pass, AttnArgs a, JoinArgs j, int64_t num_split, bool aligned, hipStream_t s) {
     constexpr int VEC = sizeof(T) == 4 ? 4 : 8;
-    const bool ok = aligned ? launch_attention_vec<T, TG, VEC, true>(pass, a, s) : launch_attention_vec<T, TG, VEC, false>(pass, a, s);
+    constexpr bool kScaled = RowScale<T>::kScaled;
+    const int heads = pass == kPassKeyValue ? a.kv_heads : a.heads;
+    a.tiles = static_cast<int>(ceil_div(heads, 1 << a.tile_log));
+    const bool ok = a.dim < VEC ? launch_attention_lanes<T, TG, VEC, 1, kSingle>(pass, a, s)
+                    : aligned   ? launch_attention_vec<T, TG, VEC, kWhole>(pass, a, s)
+                                : launch_attention_vec<T, TG, VEC, kShifted>(pass, a, s);
     if (!ok) return false;
     if (num_split == 0) return true;
-    const int64_t blocks = num_split * j.heads;
+    j.heads = heads;
+    j.windows = static_cast<int>(ceil_div(static_cast<int64_t>(heads) * a.dim, 64));
+    const int64_t blocks = num_split * j.windows;
     if (blocks > 0x7fffffffLL) return false;
     const dim3 grid(static_cast<uint32_t>(blocks)), block(256);
     if (pass == kPassForward)
-        hipLaunchKernelGGL((attn_join_kernel<TG, kJoinForward>), grid, block, 0, s, j);
+        hipLaunchKernelGGL((attn_join_kernel<TG, kJoinForward, kScaled>), grid, block, 0, s, j);
     else if (pass == kPassQuery)
-        hipLaunchKernelGGL((attn_join_kernel<TG, kJoinQuery>), grid, block, 0, s, j);
+        hipLaunchKernelGGL((attn_join_kernel<TG, kJoinQuery, kScaled>), grid, block, 0, s, j);
     else
-        hipLaunchKernelGGL((attn_join_kernel<TG, kJoinKeyValue>), grid, block, 0, s, j);
+        hipLaunchKernelGGL((attn_join_kernel<TG, kJoinKeyValue, kScaled>), grid, block, 0, s, j);
     return true;
 }
 

@@ -12,17 +12,26 @@ import torch
 from torch.autograd.function import Function, once_differentiable
 
 from . import _lib
-from .checkpoint import DTYPES, need_float, on_device_of, pack
+from .checkpoint import DTYPES, need_float, on_device_of, pack_rows
 from .kernels import _L, _ptr, _stream, _workspace, check, refuse_capture
 
-ITEM_EDGES = 64  # edges of a work item at most
+
+def item_edges(edges):
+    """Edges of a work item at most, by the graph's size: the power of two from sqrt(edges) / 16 on, 16 .. 512.  Short
+    items end together and let a small graph fill the device; long ones leave less to join (forward and join in us at
+    caps 16 / 32 / 64 / 128 / 256: 4.1 k edges 10 / 12 / 16 / 24 / 35, 0.2 M 35 / 29 / 29 / 44 / 73, 1.3 M 447 / 416 /
+    410 / 401 / 415, 9.4 M 1918 / 1479 / 1311 / 1261 / 1235)."""
+    cap = 16
+    while cap < 512 and 256 * cap * cap < edges:
+        cap *= 2
+    return cap
 
 
 class AttentionItems:
     """One orientation of a graph cut into work items (``tango_attn_items`` of include/tango_hip.h)."""
 
     def __init__(self, indptr, indices, edge_ids, cap=None):
-        cap = ITEM_EDGES if cap is None else cap
+        cap = item_edges(indices.numel()) if cap is None else cap
         dev = indptr.device
         degree = indptr[1:] - indptr[:-1]
         rows = degree.numel()
@@ -92,13 +101,26 @@ def _operands(t, q, k, v):
     (t.q_row, t.q_head), (t.k_row, t.k_head), (t.v_row, t.v_head) = (x.stride()[:2] for x in (q, k, v))
 
 
-def _checkpoint_operands(t, held):
+def _hold(q, k, v):
+    """8-bit values and scales of the three tensors, a scale per row and head.  The scales of a row's keys and values
+    lie side by side, since the backward pass reads them together."""
+    scales = [torch.empty(q.shape[:2] + (1,), dtype=torch.float32, device=q.device),
+              torch.empty(k.shape[:2] + (2,), dtype=torch.float32, device=q.device)]
+    flat = [x.reshape(x.size(0), x.size(1) * x.size(2)) for x in (q, k, v)]
+    held = [pack_rows(x, q.size(2), s) for x, s in zip(flat, (scales[0][..., 0], scales[1][..., 0], scales[1][..., 1]))]
+    return held, scales
+
+
+def _checkpoint_operands(t, held, scales):
     t.checkpoint = 1
-    for name, p in zip("qkv", held):
-        setattr(t, name, _ptr(p.values))
-        setattr(t, name + "_row", p.values.stride(0) if p.values.numel() else 0)
-        setattr(t, name + "_head", p.group)
-        setattr(t, name + "_scale", _ptr(p.scale))
+    for name, x in zip("qkv", held):
+        setattr(t, name, _ptr(x))
+        setattr(t, name + "_row", x.stride(0))
+        setattr(t, name + "_head", t.dim)
+    t.q_scale_row, t.q_scale_head = scales[0].stride()[:2]
+    t.kv_scale_row, t.kv_scale_head = scales[1].stride()[:2]
+    t.q_scale, t.k_scale = _ptr(scales[0]), _ptr(scales[1])
+    t.v_scale = t.k_scale + 4 if t.k_scale else None
 
 
 class _GraphAttention(Function):
@@ -111,14 +133,14 @@ class _GraphAttention(Function):
             t = _struct(q.shape, k.shape, scale, q.dtype)
             _operands(t, q, k, v)
             ref = ctypes.byref(t)
-            ws_bytes = _L.tango_graph_attention_workspace(ref, by_dst.ref, None)
+            ws_bytes = _L.tango_graph_attention_workspace(ref, by_dst.ref, None, edge_mask is not None)
             ws = _workspace(ws_bytes, q.device)
             check(_L.tango_graph_attention_fwd(_ptr(out), ref, by_dst.ref, _ptr(edge_mask), _ptr(ws), ws_bytes, _stream()),
                   "graph_attention")
             ctx.graph, ctx.scale, ctx.held = graph, scale, None
             if any(ctx.needs_input_grad[1:4]):
                 if checkpoint:
-                    ctx.held = tuple(pack(x.reshape(x.size(0), x.size(1) * x.size(2)), x.size(2)) for x in (q, k, v))
+                    ctx.held = _hold(q, k, v)
                     ctx.shapes = q.shape, k.shape, q.dtype
                     ctx.save_for_backward(edge_mask)
                 else:
@@ -140,11 +162,11 @@ class _GraphAttention(Function):
             else:
                 q_shape, k_shape, dtype = ctx.shapes
                 t = _struct(q_shape, k_shape, ctx.scale, dtype)
-                _checkpoint_operands(t, ctx.held)
+                _checkpoint_operands(t, *ctx.held)
             grads = [torch.empty(shape, dtype=dout.dtype, device=dout.device) if need else None
                      for shape, need in zip((q_shape, k_shape, k_shape), ctx.needs_input_grad[1:4])]
             ref = ctypes.byref(t)
-            ws_bytes = _L.tango_graph_attention_workspace(ref, by_dst.ref, by_src.ref)
+            ws_bytes = _L.tango_graph_attention_workspace(ref, by_dst.ref, by_src.ref, edge_mask is not None)
             ws = _workspace(ws_bytes, dout.device)
             check(_L.tango_graph_attention_bwd(*(None if g is None else _ptr(g) for g in grads), ref, _ptr(dout),
                                                dout.stride(0), dout.stride(1), by_dst.ref, by_src.ref, _ptr(edge_mask),

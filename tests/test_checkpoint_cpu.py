@@ -20,14 +20,15 @@ def test_python_refusals():
 def test_checkpoint_abi_refusals():
     from tango_amd import _lib
     L = _lib.lib()
-    assert L.tango_pack_i8(16, 8, 16, 16, 3, 4, 8, 8, 8, None) == -2   # no such type
-    assert L.tango_pack_i8(16, 8, 16, 16, 0, -1, 8, 8, 8, None) == -1
-    assert L.tango_pack_i8(16, 8, 16, 16, 0, 4, 8, 8, 0, None) == -1   # group
-    assert L.tango_pack_i8(16, 8, 16, None, 0, 4, 8, 8, 8, None) == -1
-    assert L.tango_pack_i8(16, 4, 16, 16, 0, 4, 8, 8, 8, None) == -1   # rows of the result overlap
-    assert L.tango_pack_i8(16, 8, 16, 18, 0, 4, 8, 8, 8, None) == -1   # fp32 off its alignment
-    assert L.tango_pack_i8(16, 8, 16, 16, 0, 4, 1 << 30, 1 << 30, 8, None) == -2
-    assert L.tango_pack_i8(None, 8, None, None, 0, 0, 8, 8, 8, None) == 0
+    assert L.tango_pack_i8(16, 8, 16, 1, 1, 16, 3, 4, 8, 8, 8, None) == -2   # no such type
+    assert L.tango_pack_i8(16, 8, 16, 1, 1, 16, 0, -1, 8, 8, 8, None) == -1
+    assert L.tango_pack_i8(16, 8, 16, 1, 1, 16, 0, 4, 8, 8, 0, None) == -1   # group
+    assert L.tango_pack_i8(16, 8, 16, 1, 1, None, 0, 4, 8, 8, 8, None) == -1
+    assert L.tango_pack_i8(16, 4, 16, 1, 1, 16, 0, 4, 8, 8, 8, None) == -1   # rows of the result overlap
+    assert L.tango_pack_i8(16, 8, 16, 1, 1, 18, 0, 4, 8, 8, 8, None) == -1   # fp32 off its alignment
+    assert L.tango_pack_i8(16, 8, 16, 1, 1, 16, 0, 4, 1 << 30, 1 << 30, 8, None) == -2
+    assert L.tango_pack_i8(None, 8, None, 1, 1, None, 0, 0, 8, 8, 8, None) == 0
+    assert L.tango_pack_i8(16, 8, 16, -1, 1, 16, 0, 4, 8, 8, 8, None) == -1
     assert L.tango_unpack_i8(16, 0, 4, 16, 8, 16, 4, 8, 8, None) == -1
     assert L.tango_unpack_i8(16, 7, 8, 16, 8, 16, 4, 8, 8, None) == -2
     assert L.tango_unpack_i8(None, 0, 8, None, 8, None, 4, 0, 8, None) == 0
@@ -75,8 +76,10 @@ def test_attention_backward_abi_refusals():
     assert L.tango_graph_attention_bwd(16, 16, 16, refs[0], 16, 16, 8, refs[1], refs[1], None, None, 0, None) == -4
     assert L.tango_graph_attention_bwd(None, None, None, refs[0], 16, 16, 8, refs[1], refs[1], None, None, 0, None) == 0
     assert L.tango_graph_attention_fwd(None, refs[0], refs[1], None, None, 0, None) == -1
-    assert L.tango_graph_attention_workspace(refs[0], refs[1], None) == 0  # no row is cut
-    assert L.tango_graph_attention_workspace(refs[0], refs[1], refs[1]) >= 4 * 2 * 8  # two floats a destination and head
+    assert L.tango_graph_attention_workspace(refs[0], refs[1], None, 0) == 0  # no row is cut
+    assert L.tango_graph_attention_workspace(refs[0], refs[1], None, 1) >= 5 * 4
+    assert L.tango_graph_attention_fwd(16, refs[0], refs[1], 16, None, 0, None) == -4
+    assert L.tango_graph_attention_workspace(refs[0], refs[1], refs[1], 0) >= 4 * 2 * 8  # two floats a destination and head
 
 
 @pytest.mark.parametrize("cap", [1, 3, 64])

@@ -321,6 +321,24 @@ def test_only_some_inputs_need_gradients(which):
     assert not graph_attention(g, *x[:3]).requires_grad
 
 
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+@pytest.mark.parametrize("t,heads,kv", [("fp32", 8, 8), ("fp32", 8, 2), ("bf16", 20, 20)])
+def test_rows_beyond_the_caches(t, heads, kv, checkpoint):
+    """Tensors larger than the L2s together: the other order of workgroups, wider tiles."""
+    from tango_amd.checkpoint import pack, unpack
+    rng = np.random.default_rng(77)
+    n, m, D = 22000, 40000, 32
+    src, dst = powerlaw_graph(rng, n, m)
+    g = make_graph(src, dst, n, n)
+    x = inputs(n, n, heads, kv, D, TYPES[t], seed=7)
+    got = run(g, *x, checkpoint=checkpoint)
+    held = x[:3] if checkpoint is None else [unpack(pack(a.flatten(1), D), torch.float32).view_as(a) for a in x[:3]]
+    want, bound = formulas(src, dst, *held, x[3], 1 / math.sqrt(D), None)
+    if checkpoint:
+        got[0], want[0], bound[0] = got[1], want[1], bound[1]  # the output is not that of the held values
+    check(got, want, bound, TYPES[t])
+
+
 def test_same_bits_every_time():
     """No result depends on the order in which workgroups run."""
     rng = np.random.default_rng(30)
