@@ -610,8 +610,8 @@ int tango_pack_i8(int8_t* q, int64_t ldq, float* scale, int64_t scale_row, int64
 int tango_unpack_i8(void* x, int dtype, int64_t ldx, const int8_t* q, int64_t ldq, const float* scale,
                     int64_t rows, int64_t cols, int64_t group, tango_stream_t stream);
 
-/* Gradients of a linear layer's weight and bias from the 8-bit checkpoint of its input (q, scale, group as
-   tango_pack_i8 wrote them; ldq a multiple of 4 is the fast case):
+/* Gradients of a linear layer's weight and bias from the 8-bit checkpoint of its input (q [M, ldq], scale [M, runs] and
+   group as of tango_pack_i8; every row of q is readable to ldq.  ldq, group and q multiples of 4 are the fast case):
      dw[n, k] = sum_m dy[m, n] * (q[m, k] * scale[m, k / group]),   db[n] = sum_m dy[m, n]  (db may be NULL)
    for dy [M, N] (dtype, row stride ldy) and q [M, K]; dw [N, K] and db [N] in dtype, contiguous.  Sums are fp32 in a
    fixed order; a row's dy * scale is held in three (fp32) or two (bf16, fp16) bf16 terms.  A dy that is not finite

@@ -6,13 +6,18 @@
 // rounding, is split into bf16 terms (each the rounding of what the ones before left): three terms hold all 24 bits of
 // an fp32 product, two (16 bits, an error of 2^-17 at most) are well below the rounding of a 16-bit result.  Sums are fp32.
 //
-// A workgroup owns a tile of kTileN x kTileK results inside one run and a share of the rows, kStep rows at a time: every
-// thread loads eight rows of a column (so the transposition that the matrix instructions want costs nothing), scales,
-// splits and writes 16 bytes of eight consecutive rows per term to LDS; four waves own a quarter of the tile each.
-// The next step's loads are in flight while a step is multiplied.  LDS is laid out [row octet][column][8 rows]: both the
-// writes and the fragment reads of neighbouring lanes are neighbouring 16-byte pieces.  Partial sums of the row shares
-// go to a slab each and a second kernel adds the slabs in order.  The tiles of one row share are neighbours on one XCD,
-// so dy and q come from HBM once and from that XCD's L2 for the other tiles.
+// A workgroup owns a tile of kTileN x at most kTileK results inside one run and a share of the rows, kStep rows at a
+// time.  Each of its four waves loads eight rows (so their scales are scalar), a lane two columns of dy and four of q;
+// a thread holds eight rows of a column, so the transposition that the matrix instructions want costs nothing, and
+// writes 16 bytes of eight consecutive rows per column and term to LDS.  Then each wave multiplies 32 of the tile's
+// dy columns with all of its q columns: 32x32x16, accumulators in registers.  The next step's loads are in flight while
+// a step is multiplied, and two workgroups a CU overlap one's conversions with the other's matrix instructions.
+// LDS is laid out [row octet][column][8 rows]: writes and fragment reads of neighbouring lanes are neighbouring 16-byte
+// pieces.  Partial sums of the row shares go to a slab each and a second kernel adds the slabs in order.  The tiles of
+// one row share are neighbours on one XCD, so dy and q come from HBM once and from that XCD's L2 for the other tiles.
+//
+// Why 128 x 256: a dy element is scaled and split (8 VALU instructions) once per tile of q columns, which at 128 x 128
+// was more than the matrix instructions it feeds (MMM).
 #include "element.hpp"
 
 namespace tango {
@@ -20,7 +25,7 @@ namespace tango {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kTileN = 128, kTileK = 128, kStep = 32;
+constexpr int kTileN = 128, kTileK = 256, kStep = 32, kSub = 32;
 
 struct WGradArgs {
     const void* dy;
@@ -28,31 +33,43 @@ struct WGradArgs {
     const float* scale;
     float *slab, *slab_b;  // [splits, N, K], [splits, N]
     int64_t ldy, ldq, M, m_share;
-    int N, K, group, runs, tiles_run, tiles_k, tiles, splits;
-    int pairs, quads;  // dy in 2-element loads (16-bit types), q in 4-byte loads
+    int N, K, group, runs, tile_k, tiles_run, tiles_k, tiles, splits;
 };
 
-// The column order inside a tile's LDS rows: what one thread loads together lies kTile / width apart, so that the
-// writes of neighbouring threads are neighbours.
-template <int WIDTH, int TILE>
-__device__ __forceinline__ int column_of(int slot) {
-    return (slot % (TILE / WIDTH)) * WIDTH + slot / (TILE / WIDTH);
-}
-
 __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
-    const uint32_t lo = __builtin_bit_cast(uint16_t, static_cast<bf16_t>(a));
-    const uint32_t hi = __builtin_bit_cast(uint16_t, static_cast<bf16_t>(b));
-    return lo | (hi << 16);
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const f32x2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
 }
 
-template <typename T, int TERMS>
-__global__ __launch_bounds__(256) void weight_grad_kernel(const WGradArgs a) {
-    constexpr int W = sizeof(T) == 4 ? 1 : 2;               // columns of dy a thread loads together
-    constexpr int ITEMS = kTileN / W * (kStep / 8) / 256;   // (columns, octet) pieces per thread
-    __shared__ u32x4 lds_a[2][TERMS][kStep / 8][kTileN];
-    __shared__ u32x4 lds_b[2][kStep / 8][kTileK];
+// Columns and slots.  Slot 64 w + l of a dy row holds column 2 l + w (a lane writes its columns 2 l and 2 l + 1 beside its
+// neighbours'); the smallest column of the 32 slots from s on is that of s.
+__device__ __forceinline__ int n_column(int slot) { return 2 * (slot & 63) + (slot >> 6); }
+// Column 4 l + j of a q row, in pieces of 64 slots for each j.  A fragment of 32 neighbouring columns reads eight slots of
+// each piece; every other piece is turned by eight slots (128 bytes), so that two pieces read together lie in different
+// banks.
+__device__ __forceinline__ int k_slot(int j, int l) { return j * 64 + (l ^ ((j & 1) << 3)); }
+__device__ __forceinline__ int k_column(int sub, int col) { return kSub * sub + 4 * (col & 7) + (col >> 3); }
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// A wave's eight rows of one step in registers.
+template <typename T>
+struct WGradStage {
+    Pack<T, 2> dy[8];
+    uint32_t q[8];
+    float scale;  // lane l: that of row l % 8
+};
+
+// WHOLE: dy in loads of two columns (N > 1), q in loads of four (runs and rows of q start on multiples of four), both
+// unconditional: columns past the end are moved back inside, what they give is not used.  Otherwise an element at a time.
+template <typename T, int TERMS, int SUBS, bool WHOLE>
+__global__ __launch_bounds__(256, 2) void weight_grad_kernel(const WGradArgs a) {
+    // [buffer][term, then q][octet][column]
+    constexpr int kA = TERMS * (kStep / 8) * kTileN, kB = (kStep / 8) * kTileK;
+    extern __shared__ u32x4 lds[];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int split, tile;
     if (a.splits >= 8) {  // a split's tiles stay on one XCD
         const int j = blockIdx.x >> 3;
@@ -66,166 +83,207 @@ __global__ __launch_bounds__(256) void weight_grad_kernel(const WGradArgs a) {
     const int tk = tile % a.tiles_k, n0 = tile / a.tiles_k * kTileN;
     const int run = tk / a.tiles_run;
     const int run_end = run == a.runs - 1 ? a.K : (run + 1) * a.group;
-    const int k0 = run * a.group + (tk - run * a.tiles_run) * kTileK;
-    const int k_end = k0 + kTileK < run_end ? k0 + kTileK : run_end;
+    const int k0 = run * a.group + (tk - run * a.tiles_run) * a.tile_k;
+    const int k_end = k0 + a.tile_k < run_end ? k0 + a.tile_k : run_end;
     const int64_t m_begin = split * a.m_share;
     const int64_t m_end = m_begin + a.m_share < a.M ? m_begin + a.m_share : a.M;
     const bool want_b = a.slab_b && tk == 0;
 
-    const T* dy = static_cast<const T*>(a.dy);
-    Pack<T, W> ra[ITEMS][8];
-    float rs[ITEMS][8];
-    uint32_t rq[4];
-    float bsum[ITEMS][W];
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-        for (int w = 0; w < W; ++w) bsum[i][w] = 0.0f;
+    // This lane's columns.  If N is odd, the lane of the last column loads the pair that ends with it, one column early.
+    const int n = n0 + 2 * lane, k = k0 + 4 * lane;
+    const int n_at = n + 1 < a.N ? n : a.N - 2, k_at = k < k_end ? k : k0;
 
-    // this thread's pieces: dy columns and octet, q columns and half octet
-    int col[ITEMS], oct[ITEMS];
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const int id = tid + 256 * i;
-        col[i] = id % (kTileN / W);
-        oct[i] = id / (kTileN / W);
-    }
-    const int kc = tid % (kTileK / 4), mq = tid / (kTileK / 4);
-    const int kq = k0 + 4 * kc;
+    float bsum[2] = {0.0f, 0.0f};
 
-    auto load = [&](int64_t m0) {
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int n = n0 + col[i] * W;
+    // the wave's eight rows from `first` on; rows past `last` are that row again, and convert() drops them
+    auto load = [&](WGradStage<T>& st, int64_t first, int last) {
+        const T* dy = static_cast<const T*>(a.dy) + first * a.ldy;
+        const int8_t* q = a.q + first * a.ldq;
+        if constexpr (WHOLE) {
+            typedef uint32_t U4 __attribute__((aligned(1)));
+            typedef u32x2 U8 __attribute__((aligned(1)));
+            const uint32_t dy_at = static_cast<uint32_t>(n_at) * sizeof(T), q_at = static_cast<uint32_t>(k_at);
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-                const int64_t m = m0 + oct[i] * 8 + r;
-                const bool ok = m < m_end && n < a.N;
-                ra[i][r].zero();
-                rs[i][r] = 0.0f;
-                if (ok) {
-                    const T* p = dy + m * a.ldy + n;
-                    if constexpr (W == 1) {
-                        ra[i][r].load(p);
-                    } else if (a.pairs && n + 1 < a.N) {
-                        ra[i][r].load(p);
-                    } else {
-                        const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-                        ra[i][r].w[0] = h[0] | (n + 1 < a.N ? static_cast<uint32_t>(h[1]) << 16 : 0u);
-                    }
-                    rs[i][r] = a.scale[m * a.runs + run];
+                const int row = r < last ? r : last;
+                const char* p = reinterpret_cast<const char*>(dy + row * a.ldy) + dy_at;
+                if constexpr (sizeof(T) == 4) {
+                    const u32x2 t = *reinterpret_cast<const U8*>(p);
+                    st.dy[r].w[0] = t[0];
+                    st.dy[r].w[1] = t[1];
+                } else {
+                    st.dy[r].w[0] = *reinterpret_cast<const U4*>(p);
                 }
+                st.q[r] = *reinterpret_cast<const uint32_t*>(q + row * a.ldq + q_at);
+            }
+        } else {
+            for (int r = 0; r < 8; ++r) {
+                const int row = r < last ? r : last;
+                Pack<T, 1> x, y;
+                x.zero();
+                y.zero();
+                if (n < a.N) x.load(dy + row * a.ldy + n);
+                if (n + 1 < a.N) y.load(dy + row * a.ldy + n + 1);
+                uint32_t w = 0;
+                for (int j = 0; j < 4; ++j)
+                    if (k + j < k_end) w |= static_cast<uint32_t>(static_cast<uint8_t>(q[row * a.ldq + k + j])) << (8 * j);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i == r) {
+                        if constexpr (sizeof(T) == 4) {
+                            st.dy[i].w[0] = x.w[0];
+                            st.dy[i].w[1] = y.w[0];
+                        } else {
+                            st.dy[i].w[0] = x.w[0] | (y.w[0] << 16);
+                        }
+                        st.q[i] = w;
+                    }
             }
         }
+        // one vector load: scalar loads share a counter with the LDS reads that the matrix instructions wait for
+        const int sr = (lane & 7) < last ? (lane & 7) : last;
+        st.scale = a.scale[(first + sr) * a.runs + run];
+    };
+    auto convert_dy = [&](const WGradStage<T>& st, u32x4* at, int rows) {
+        float scale[8];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int64_t m = m0 + mq * 4 + r;
-            rq[r] = 0;
-            if (m < m_end && kq < k_end) {
-                const int8_t* p = a.q + m * a.ldq + kq;
-                if (a.quads && kq + 3 < a.K) {
-                    rq[r] = *reinterpret_cast<const uint32_t*>(p);
-                } else {
+        for (int r = 0; r < 8; ++r) scale[r] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(st.scale), r));
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (kq + j < k_end) rq[r] |= static_cast<uint32_t>(static_cast<uint8_t>(p[j])) << (8 * j);
+        for (int w = 0; w < 2; ++w) {
+            float x[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) x[r] = r < rows ? st.dy[r].get(w) : 0.0f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) bsum[w] += x[r];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) x[r] = r < rows ? x[r] * scale[r] : 0.0f;
+#pragma unroll
+            for (int t = 0; t < TERMS; ++t) {
+                u32x4 o;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    o[p] = bf16_pair(x[2 * p], x[2 * p + 1]);
+                    x[2 * p] -= __uint_as_float(o[p] << 16);
+                    x[2 * p + 1] -= __uint_as_float(o[p] & 0xffff0000u);
                 }
+                at[(t * (kStep / 8) + wave) * kTileN + w * 64 + lane] = o;
             }
         }
     };
-    auto store = [&](int buf, int64_t m0) {
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                float x[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    const float d = ra[i][r].get(w);
-                    bsum[i][w] += d;
-                    // rows past the end hold zeros, whatever their scale
-                    x[r] = m0 + oct[i] * 8 + r < m_end ? d * rs[i][r] : 0.0f;
-                }
-#pragma unroll
-                for (int t = 0; t < TERMS; ++t) {
-                    u32x4 o;
-#pragma unroll
-                    for (int p = 0; p < 4; ++p) {
-                        o[p] = bf16_pair(x[2 * p], x[2 * p + 1]);
-                        x[2 * p] -= __uint_as_float(o[p] << 16);
-                        x[2 * p + 1] -= __uint_as_float(o[p] & 0xffff0000u);
-                    }
-                    lds_a[buf][t][oct[i]][w * (kTileN / W) + col[i]] = o;
-                }
-            }
+    auto convert_q = [&](const WGradStage<T>& st, u32x4* at) {
+        // (lanes past SUBS * kSub columns write slots that nothing reads)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float x[4];
+            float x[8];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = static_cast<float>(static_cast<int8_t>(rq[r] >> (8 * j)));
-            u32x2 o;
-            o[0] = bf16_pair(x[0], x[1]);
-            o[1] = bf16_pair(x[2], x[3]);
-            reinterpret_cast<u32x2*>(&lds_b[buf][mq >> 1][j * (kTileK / 4) + kc])[mq & 1] = o;
+            for (int r = 0; r < 8; ++r) x[r] = static_cast<float>(static_cast<int8_t>(st.q[r] >> (8 * j)));
+            u32x4 o;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) o[p] = bf16_pair(x[2 * p], x[2 * p + 1]);
+            at[kA + wave * kTileK + k_slot(j, lane)] = o;
         }
     };
 
-    f32x16 acc[2][2];
+    f32x16 acc[SUBS];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < SUBS; ++j)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int r = 0; r < 16; ++r) acc[j][r] = 0.0f;
+    const int half = lane >> 5, col = lane & 31;
+    auto multiply = [&](const u32x4* at, int s) {
+        bf16x8 fa[TERMS], fb[SUBS];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    const int wn = (wave >> 1) * 64 + (lane & 31), wk = (wave & 1) * 64 + (lane & 31), half = lane >> 5;
-
-    if (m_begin < m_end) {
-        load(m_begin);
-        store(0, m_begin);
-    }
-    __syncthreads();
-    int buf = 0;
-    for (int64_t m0 = m_begin; m0 < m_end; m0 += kStep) {
-        const bool more = m0 + kStep < m_end;
-        if (more) load(m0 + kStep);
+        for (int t = 0; t < TERMS; ++t)
+            fa[t] = __builtin_bit_cast(bf16x8, at[(t * (kStep / 8) + 2 * s + half) * kTileN + wave * 32 + col]);
 #pragma unroll
-        for (int s = 0; s < kStep / 16; ++s) {
-            bf16x8 fb[2];
+        for (int j = 0; j < SUBS; ++j)
+            fb[j] = __builtin_bit_cast(bf16x8, at[kA + (2 * s + half) * kTileK + k_slot(col >> 3, 8 * j + (col & 7))]);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) fb[j] = __builtin_bit_cast(bf16x8, lds_b[buf][2 * s + half][wk + 32 * j]);
+        for (int t = 0; t < TERMS; ++t)
 #pragma unroll
-            for (int t = 0; t < TERMS; ++t)
+            for (int j = 0; j < SUBS; ++j) acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[t], fb[j], acc[j], 0, 0, 0);
+    };
+    // Order of issue inside a half step: the fragment reads, then a few vector instructions behind each matrix instruction.
+    auto interleave = [&]() {
+        __builtin_amdgcn_sched_group_barrier(0x100, TERMS + SUBS, 0);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const bf16x8 fa = __builtin_bit_cast(bf16x8, lds_a[buf][t][2 * s + half][wn + 32 * i]);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa, fb[j], acc[i][j], 0, 0, 0);
-                }
+        for (int m = 0; m < TERMS * SUBS; ++m) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 7, 0);
         }
-        if (more) store(buf ^ 1, m0 + kStep);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    // Whole steps: while step i is multiplied, step i + 1 is converted into the other buffer (in the same stretch of code:
+    // vector and matrix instructions of a wave overlap) and the loads of step i + 2 are on their way.
+    const int steps = static_cast<int>((m_end - m_begin) / kStep);
+    const int64_t m_wave = m_begin + wave * 8;
+    u32x4 *const buf0 = lds, *const buf1 = lds + kA + kB;
+    if (steps > 0) {
+        WGradStage<T> s0, s1;
+        auto step = [&](WGradStage<T>& loading, const WGradStage<T>& loaded, const u32x4* now, u32x4* next, int i) {
+            load(loading, m_wave + static_cast<int64_t>(i + 2 < steps ? i + 2 : steps - 1) * kStep, 7);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(now, 0);
+            convert_dy(loaded, next, 8);
+            interleave();
+            multiply(now, 1);
+            convert_q(loaded, next);
+            interleave();
+            __syncthreads();
+        };
+        load(s0, m_wave, 7);
+        load(s1, m_wave + static_cast<int64_t>(steps > 1 ? 1 : 0) * kStep, 7);
+        convert_dy(s0, buf0, 8);
+        convert_q(s0, buf0);
         __syncthreads();
-        buf ^= 1;
+        int i = 0;
+        for (; i + 2 < steps; i += 2) {
+            step(s0, s1, buf0, buf1, i);
+            step(s1, s0, buf1, buf0, i + 1);
+        }
+        if (i + 1 < steps) {
+            step(s0, s1, buf0, buf1, i);
+            multiply(buf1, 0);
+            multiply(buf1, 1);
+        } else {
+            multiply(buf0, 0);
+            multiply(buf0, 1);
+        }
+        __syncthreads();
+    }
+    const int64_t m_rest = m_wave + static_cast<int64_t>(steps) * kStep;
+    if (m_begin + static_cast<int64_t>(steps) * kStep < m_end) {  // the last rows of all
+        const int rows = m_end - m_rest >= 8 ? 8 : m_end - m_rest > 0 ? static_cast<int>(m_end - m_rest) : 0;
+        WGradStage<T> s0;
+        load(s0, rows > 0 ? m_rest : m_end - 1, rows > 0 ? rows - 1 : 0);
+        convert_dy(s0, buf0, rows);
+        convert_q(s0, buf0);
+        __syncthreads();
+        multiply(buf0, 0);
+        multiply(buf0, 1);
+        __syncthreads();
     }
 
+    // what slot s holds: with an odd N the last lane's two slots hold the columns before and at the end
+    auto result_column = [&](int s) {
+        const int c = n0 + n_column(s);
+        return WHOLE && (a.N & 1) && (c | 1) == a.N ? c - 1 : c;
+    };
     float* slab = a.slab + static_cast<int64_t>(split) * a.N * a.K;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < SUBS; ++j)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int sn = (wave >> 1) * 64 + 32 * i + 8 * (r / 4) + 4 * half + (r & 3);
-                const int n = n0 + column_of<W, kTileN>(sn);
-                const int k = k0 + column_of<4, kTileK>(wk + 32 * j);
-                if (n < a.N && k < k_end) slab[static_cast<int64_t>(n) * a.K + k] = acc[i][j][r];
-            }
+        for (int r = 0; r < 16; ++r) {
+            const int nn = result_column(wave * 32 + 8 * (r / 4) + 4 * half + (r & 3));
+            const int kk = k0 + k_column(j, col);
+            if (nn < a.N && kk < k_end) slab[static_cast<int64_t>(nn) * a.K + kk] = acc[j][r];
+        }
     if (want_b) {  // the octets' sums of a column, in octet order
-        float* sums = reinterpret_cast<float*>(lds_a);
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-            for (int w = 0; w < W; ++w) sums[oct[i] * kTileN + col[i] * W + w] = bsum[i][w];
+        float* sums = reinterpret_cast<float*>(lds);
+        const bool early = WHOLE && n == a.N - 1;
+        sums[wave * kTileN + 2 * lane] = early ? bsum[1] : bsum[0];
+        sums[wave * kTileN + 2 * lane + 1] = bsum[1];
         __syncthreads();
         if (tid < kTileN && n0 + tid < a.N) {
             float t = 0.0f;
@@ -255,19 +313,21 @@ __global__ __launch_bounds__(256) void weight_grad_sum_kernel(T* dw, T* db, cons
 }
 
 struct WGradPlan {
-    int64_t runs, tiles_run, tiles_k, tiles, splits, m_share, slab_floats;
+    int64_t runs, tile_k, tiles_run, tiles_k, tiles, splits, m_share, slab_floats;
 };
 
 static WGradPlan wgrad_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
     WGradPlan p;
     if (group > K) group = K;
     p.runs = ceil_div(K, group);
-    p.tiles_run = ceil_div(group, kTileK);
+    // a run in equal tiles
+    p.tile_k = ceil_div(ceil_div(group, ceil_div(group, kTileK)), kSub) * kSub;
+    p.tiles_run = ceil_div(group, p.tile_k);
     const int64_t last = K - (p.runs - 1) * group;
-    p.tiles_k = (p.runs - 1) * p.tiles_run + ceil_div(last, kTileK);
+    p.tiles_k = (p.runs - 1) * p.tiles_run + ceil_div(last, p.tile_k);
     p.tiles = p.tiles_k * ceil_div(N, kTileN);
-    // two workgroups for each CU, each at least four steps of rows
-    int64_t splits = ceil_div(512, p.tiles);
+    // as many as are resident together (two a CU), no second round; each at least four steps of rows
+    int64_t splits = 512 / p.tiles;
     const int64_t most = ceil_div(M, 4 * kStep);
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
@@ -277,13 +337,41 @@ static WGradPlan wgrad_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
     return p;
 }
 
-template <typename T, int TERMS>
-static void launch_weight_grad(const WGradArgs& a, void* dw, void* db, hipStream_t s) {
+template <typename T, int TERMS, int SUBS, bool WHOLE>
+static bool launch_weight_grad_tile(const WGradArgs& a, hipStream_t s) {
+    constexpr int kLds = 2 * (kStep / 8) * (TERMS * kTileN + kTileK) * 16;  // 80 KB with three terms: two workgroups a CU
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(weight_grad_kernel<T, TERMS, SUBS, WHOLE>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess) {
+        (void)hipGetLastError();
+        return false;
+    }
     const int64_t blocks = static_cast<int64_t>(a.splits >= 8 ? (a.splits + 7) / 8 * 8 : a.splits) * a.tiles;
-    hipLaunchKernelGGL((weight_grad_kernel<T, TERMS>), dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((weight_grad_kernel<T, TERMS, SUBS, WHOLE>), dim3(static_cast<uint32_t>(blocks)), dim3(256), kLds, s, a);
+    return true;
+}
+
+template <typename T, int TERMS>
+static bool launch_weight_grad(const WGradArgs& a, bool whole, void* dw, void* db, hipStream_t s) {
+    bool ok = false;
+    if (!whole) {
+        ok = launch_weight_grad_tile<T, TERMS, kTileK / kSub, false>(a, s);
+    } else {
+        switch (a.tile_k / kSub) {
+            case 1: ok = launch_weight_grad_tile<T, TERMS, 1, true>(a, s); break;
+            case 2: ok = launch_weight_grad_tile<T, TERMS, 2, true>(a, s); break;
+            case 3: ok = launch_weight_grad_tile<T, TERMS, 3, true>(a, s); break;
+            case 4: ok = launch_weight_grad_tile<T, TERMS, 4, true>(a, s); break;
+            case 5: ok = launch_weight_grad_tile<T, TERMS, 5, true>(a, s); break;
+            case 6: ok = launch_weight_grad_tile<T, TERMS, 6, true>(a, s); break;
+            case 7: ok = launch_weight_grad_tile<T, TERMS, 7, true>(a, s); break;
+            case 8: ok = launch_weight_grad_tile<T, TERMS, 8, true>(a, s); break;
+        }
+    }
+    if (!ok) return false;
     const int64_t count = static_cast<int64_t>(a.N) * a.K;
     hipLaunchKernelGGL((weight_grad_sum_kernel<T>), dim3(static_cast<uint32_t>(ceil_div(count + (db ? a.N : 0), 256))), dim3(256), 0, s,
                        static_cast<T*>(dw), static_cast<T*>(db), a.slab, a.slab_b, count, a.N, a.splits);
+    return true;
 }
 
 // sizes whose tile counts and offsets into a slab stay within the kernels' 32-bit numbers
@@ -329,19 +417,16 @@ int tango_weight_grad_i8(void* dw, void* db, const void* dy, int dtype, int64_t 
     a.K = static_cast<int>(K);
     a.group = static_cast<int>(group > K ? K : group);
     a.runs = static_cast<int>(p.runs);
+    a.tile_k = static_cast<int>(p.tile_k);
     a.tiles_run = static_cast<int>(p.tiles_run);
     a.tiles_k = static_cast<int>(p.tiles_k);
     a.tiles = static_cast<int>(p.tiles);
     a.splits = static_cast<int>(p.splits);
-    a.pairs = ldy % 2 == 0 && aligned_to(dy, 4);
-    a.quads = ldq % 4 == 0 && aligned_to(q, 4) && (p.runs == 1 || group % 4 == 0);
-    if (dtype == TANGO_F32)
-        launch_weight_grad<float, 3>(a, dw, db, as_stream(stream));
-    else if (dtype == TANGO_BF16)
-        launch_weight_grad<bf16_t, 2>(a, dw, db, as_stream(stream));
-    else
-        launch_weight_grad<f16_t, 2>(a, dw, db, as_stream(stream));
-    return launch_status();
+    const bool whole = N > 1 && ldq % 4 == 0 && ldq >= ceil_div(K, 4) * 4 && aligned_to(q, 4) && (p.runs == 1 || group % 4 == 0);
+    const bool ok = dtype == TANGO_F32    ? launch_weight_grad<float, 3>(a, whole, dw, db, as_stream(stream))
+                    : dtype == TANGO_BF16 ? launch_weight_grad<bf16_t, 2>(a, whole, dw, db, as_stream(stream))
+                                          : launch_weight_grad<f16_t, 2>(a, whole, dw, db, as_stream(stream));
+    return ok ? launch_status() : TANGO_ERR_LAUNCH;
 }
 
 }  // extern "C"
