@@ -46,10 +46,14 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
 // Columns and slots.  Slot 64 w + l of a dy row holds column 2 l + w (a lane writes its columns 2 l and 2 l + 1 beside its
 // neighbours'); the smallest column of the 32 slots from s on is that of s.
 __device__ __forceinline__ int n_column(int slot) { return 2 * (slot & 63) + (slot >> 6); }
-// Column 4 l + j of a q row, in pieces of 64 slots for each j.  A fragment of 32 neighbouring columns reads eight slots of
-// each piece; every other piece is turned by eight slots (128 bytes), so that two pieces read together lie in different
-// banks.
-__device__ __forceinline__ int k_slot(int j, int l) { return j * 64 + (l ^ ((j & 1) << 3)); }
+// Column 4 l + j of a q row, in a piece of 8 SUBS slots for each j.  A fragment of 32 neighbouring columns reads eight
+// slots (128 bytes) of each piece; pieces read together lie in different banks (256 bytes) if an odd piece starts on an
+// odd multiple of 128 bytes: for an odd SUBS it does, else it is turned by eight slots.
+template <int SUBS>
+__device__ __forceinline__ int k_slot(int j, int l) {
+    if constexpr (SUBS % 2 == 0) l = l + 8 * (j & 1) < 8 * SUBS ? l + 8 * (j & 1) : l + 8 - 8 * SUBS;
+    return j * (8 * SUBS) + l;
+}
 __device__ __forceinline__ int k_column(int sub, int col) { return kSub * sub + 4 * (col & 7) + (col >> 3); }
 
 // A wave's eight rows of one step in registers.
@@ -60,12 +64,30 @@ struct WGradStage {
     float scale;  // lane l: that of row l % 8
 };
 
+// A load whose base is the same in all lanes and stays in scalar registers, plus a 32-bit offset per lane (left alone, the
+// compiler adds the lane's offset first and holds sixteen 64-bit addresses in vector registers).
+template <typename V, typename P>
+__device__ __forceinline__ V load_from(const P* base, uint32_t offset) {
+    typedef const V __attribute__((address_space(1), aligned(1))) * Global;
+    uint64_t at = reinterpret_cast<uint64_t>(base);
+    asm("" : "+s"(at));
+    return *reinterpret_cast<Global>(at + offset);
+}
+
+// One for a row that is there, zero for one that is not: a scalar, which the compiler is not to turn into a selection in
+// every lane.
+__device__ __forceinline__ float presence(bool there) {
+    uint32_t b = there ? 0x3f800000u : 0u;
+    asm("" : "+s"(b));
+    return __uint_as_float(b);
+}
+
 // WHOLE: dy in loads of two columns (N > 1), q in loads of four (runs and rows of q start on multiples of four), both
 // unconditional: columns past the end are moved back inside, what they give is not used.  Otherwise an element at a time.
 template <typename T, int TERMS, int SUBS, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void weight_grad_kernel(const WGradArgs a) {
     // [buffer][term, then q][octet][column]
-    constexpr int kA = TERMS * (kStep / 8) * kTileN, kB = (kStep / 8) * kTileK;
+    constexpr int kA = TERMS * (kStep / 8) * kTileN, kB = (kStep / 8) * SUBS * kSub;
     extern __shared__ u32x4 lds[];
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -95,26 +117,23 @@ __global__ __launch_bounds__(256, 2) void weight_grad_kernel(const WGradArgs a) 
 
     float bsum[2] = {0.0f, 0.0f};
 
-    // the wave's eight rows from `first` on; rows past `last` are that row again, and convert() drops them
-    auto load = [&](WGradStage<T>& st, int64_t first, int last) {
+    // the wave's eight rows from `first` on; rows past `last` are that row again, and convert drops them
+    auto load_rows = [&](WGradStage<T>& st, int64_t first, int last) {
         const T* dy = static_cast<const T*>(a.dy) + first * a.ldy;
         const int8_t* q = a.q + first * a.ldq;
         if constexpr (WHOLE) {
-            typedef uint32_t U4 __attribute__((aligned(1)));
-            typedef u32x2 U8 __attribute__((aligned(1)));
             const uint32_t dy_at = static_cast<uint32_t>(n_at) * sizeof(T), q_at = static_cast<uint32_t>(k_at);
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
                 const int row = r < last ? r : last;
-                const char* p = reinterpret_cast<const char*>(dy + row * a.ldy) + dy_at;
                 if constexpr (sizeof(T) == 4) {
-                    const u32x2 t = *reinterpret_cast<const U8*>(p);
+                    const u32x2 t = load_from<u32x2>(dy + row * a.ldy, dy_at);
                     st.dy[r].w[0] = t[0];
                     st.dy[r].w[1] = t[1];
                 } else {
-                    st.dy[r].w[0] = *reinterpret_cast<const U4*>(p);
+                    st.dy[r].w[0] = load_from<uint32_t>(dy + row * a.ldy, dy_at);
                 }
-                st.q[r] = *reinterpret_cast<const uint32_t*>(q + row * a.ldq + q_at);
+                st.q[r] = load_from<uint32_t>(q + row * a.ldq, q_at);
             }
         } else {
             for (int r = 0; r < 8; ++r) {
@@ -144,19 +163,34 @@ __global__ __launch_bounds__(256, 2) void weight_grad_kernel(const WGradArgs a) 
         const int sr = (lane & 7) < last ? (lane & 7) : last;
         st.scale = a.scale[(first + sr) * a.runs + run];
     };
+    const int share = static_cast<int>(m_end - m_begin);
+    auto rows_of = [&](int step) {  // of this wave: 0 .. 8
+        const int left = share - step * kStep - wave * 8;
+        return left >= 8 ? 8 : left > 0 ? left : 0;
+    };
+    auto load = [&](WGradStage<T>& st, int step) {
+        const int64_t first = m_begin + static_cast<int64_t>(step) * kStep + wave * 8;
+        const int rows = rows_of(step);
+        if (rows == 8)
+            load_rows(st, first, 7);
+        else
+            load_rows(st, rows > 0 ? first : m_end - 1, rows > 0 ? rows - 1 : 0);
+    };
+    // Rows that are not there repeat one that is, with a scale of zero: they add nothing to a finite sum (and one that is
+    // not finite already holds that row).
     auto convert_dy = [&](const WGradStage<T>& st, u32x4* at, int rows) {
         float scale[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) scale[r] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(st.scale), r));
+        for (int r = 0; r < 8; ++r)
+            scale[r] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(st.scale), r) & (r < rows ? -1 : 0));
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             float x[8];
 #pragma unroll
-            for (int r = 0; r < 8; ++r) x[r] = r < rows ? st.dy[r].get(w) : 0.0f;
-#pragma unroll
-            for (int r = 0; r < 8; ++r) bsum[w] += x[r];
-#pragma unroll
-            for (int r = 0; r < 8; ++r) x[r] = r < rows ? x[r] * scale[r] : 0.0f;
+            for (int r = 0; r < 8; ++r) {
+                bsum[w] = __builtin_fmaf(st.dy[r].get(w), presence(r < rows), bsum[w]);
+                x[r] = st.dy[r].get(w) * scale[r];
+            }
 #pragma unroll
             for (int t = 0; t < TERMS; ++t) {
                 u32x4 o;
@@ -170,8 +204,8 @@ __global__ __launch_bounds__(256, 2) void weight_grad_kernel(const WGradArgs a) 
             }
         }
     };
+    const int k_lane = lane < 8 * SUBS ? lane : 0;
     auto convert_q = [&](const WGradStage<T>& st, u32x4* at) {
-        // (lanes past SUBS * kSub columns write slots that nothing reads)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float x[8];
@@ -180,7 +214,9 @@ __global__ __launch_bounds__(256, 2) void weight_grad_kernel(const WGradArgs a) 
             u32x4 o;
 #pragma unroll
             for (int p = 0; p < 4; ++p) o[p] = bf16_pair(x[2 * p], x[2 * p + 1]);
-            at[kA + wave * kTileK + k_slot(j, lane)] = o;
+            // lanes without a column write what nothing reads
+            u32x4* const to = at + kA + wave * (SUBS * kSub) + k_slot<SUBS>(j, k_lane);
+            *(lane < 8 * SUBS ? to : lds + 2 * (kA + kB) + (lane & 7)) = o;
         }
     };
 
@@ -197,7 +233,7 @@ __global__ __launch_bounds__(256, 2) void weight_grad_kernel(const WGradArgs a) 
             fa[t] = __builtin_bit_cast(bf16x8, at[(t * (kStep / 8) + 2 * s + half) * kTileN + wave * 32 + col]);
 #pragma unroll
         for (int j = 0; j < SUBS; ++j)
-            fb[j] = __builtin_bit_cast(bf16x8, at[kA + (2 * s + half) * kTileK + k_slot(col >> 3, 8 * j + (col & 7))]);
+            fb[j] = __builtin_bit_cast(bf16x8, at[kA + (2 * s + half) * (SUBS * kSub) + k_slot<SUBS>(col >> 3, 8 * j + (col & 7))]);
 #pragma unroll
         for (int t = 0; t < TERMS; ++t)
 #pragma unroll
@@ -214,55 +250,32 @@ __global__ __launch_bounds__(256, 2) void weight_grad_kernel(const WGradArgs a) 
         __builtin_amdgcn_sched_barrier(0);
     };
 
-    // Whole steps: while step i is multiplied, step i + 1 is converted into the other buffer (in the same stretch of code:
-    // vector and matrix instructions of a wave overlap) and the loads of step i + 2 are on their way.
-    const int steps = static_cast<int>((m_end - m_begin) / kStep);
-    const int64_t m_wave = m_begin + wave * 8;
+    // While step i is multiplied, step i + 1 is converted into the other buffer (in the same stretch of code: vector and
+    // matrix instructions of a wave overlap) and the loads of step i + 2 are on their way.  Steps in pairs: an odd
+    // number is followed by one without rows.
+    const int steps = (share + kStep - 1) / kStep;
     u32x4 *const buf0 = lds, *const buf1 = lds + kA + kB;
-    if (steps > 0) {
-        WGradStage<T> s0, s1;
-        auto step = [&](WGradStage<T>& loading, const WGradStage<T>& loaded, const u32x4* now, u32x4* next, int i) {
-            load(loading, m_wave + static_cast<int64_t>(i + 2 < steps ? i + 2 : steps - 1) * kStep, 7);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(now, 0);
-            convert_dy(loaded, next, 8);
-            interleave();
-            multiply(now, 1);
-            convert_q(loaded, next);
-            interleave();
-            __syncthreads();
-        };
-        load(s0, m_wave, 7);
-        load(s1, m_wave + static_cast<int64_t>(steps > 1 ? 1 : 0) * kStep, 7);
-        convert_dy(s0, buf0, 8);
-        convert_q(s0, buf0);
+    WGradStage<T> s0, s1;
+    auto step = [&](WGradStage<T>& loading, const WGradStage<T>& loaded, const u32x4* now, u32x4* next, int i) {
+        load(loading, i + 2);
+        const int rows = rows_of(i + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(now, 0);
+        convert_dy(loaded, next, rows);
+        interleave();
+        multiply(now, 1);
+        convert_q(loaded, next);
+        interleave();
         __syncthreads();
-        int i = 0;
-        for (; i + 2 < steps; i += 2) {
-            step(s0, s1, buf0, buf1, i);
-            step(s1, s0, buf1, buf0, i + 1);
-        }
-        if (i + 1 < steps) {
-            step(s0, s1, buf0, buf1, i);
-            multiply(buf1, 0);
-            multiply(buf1, 1);
-        } else {
-            multiply(buf0, 0);
-            multiply(buf0, 1);
-        }
-        __syncthreads();
-    }
-    const int64_t m_rest = m_wave + static_cast<int64_t>(steps) * kStep;
-    if (m_begin + static_cast<int64_t>(steps) * kStep < m_end) {  // the last rows of all
-        const int rows = m_end - m_rest >= 8 ? 8 : m_end - m_rest > 0 ? static_cast<int>(m_end - m_rest) : 0;
-        WGradStage<T> s0;
-        load(s0, rows > 0 ? m_rest : m_end - 1, rows > 0 ? rows - 1 : 0);
-        convert_dy(s0, buf0, rows);
-        convert_q(s0, buf0);
-        __syncthreads();
-        multiply(buf0, 0);
-        multiply(buf0, 1);
-        __syncthreads();
+    };
+    load(s0, 0);
+    load(s1, 1);
+    convert_dy(s0, buf0, rows_of(0));
+    convert_q(s0, buf0);
+    __syncthreads();
+    for (int i = 0; i < steps; i += 2) {
+        step(s0, s1, buf0, buf1, i);
+        step(s1, s0, buf1, buf0, i + 1);
     }
 
     // what slot s holds: with an odd N the last lane's two slots hold the columns before and at the end
@@ -326,8 +339,9 @@ static WGradPlan wgrad_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
     const int64_t last = K - (p.runs - 1) * group;
     p.tiles_k = (p.runs - 1) * p.tiles_run + ceil_div(last, p.tile_k);
     p.tiles = p.tiles_k * ceil_div(N, kTileN);
-    // as many as are resident together (two a CU), no second round; each at least four steps of rows
-    int64_t splits = 512 / p.tiles;
+    // as many as are resident together (two workgroups on each of an XCD's 32 CUs), no second round; each at least four
+    // steps of rows
+    int64_t splits = p.tiles <= 64 ? 8 * (64 / p.tiles) : 512 / p.tiles;
     const int64_t most = ceil_div(M, 4 * kStep);
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
@@ -339,7 +353,7 @@ static WGradPlan wgrad_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
 
 template <typename T, int TERMS, int SUBS, bool WHOLE>
 static bool launch_weight_grad_tile(const WGradArgs& a, hipStream_t s) {
-    constexpr int kLds = 2 * (kStep / 8) * (TERMS * kTileN + kTileK) * 16;  // 80 KB with three terms: two workgroups a CU
+    constexpr int kLds = 2 * (kStep / 8) * (TERMS * kTileN + SUBS * kSub) * 16 + (SUBS * kSub < kTileK ? 128 : 0);
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(weight_grad_kernel<T, TERMS, SUBS, WHOLE>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess) {
         (void)hipGetLastError();
