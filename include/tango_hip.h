@@ -616,7 +616,7 @@ int tango_unpack_i8(void* x, int dtype, int64_t ldx, const int8_t* q, int64_t ld
    for dy [M, N] (dtype, row stride ldy) and q [M, K]; dw [N, K] and db [N] in dtype, contiguous.  Sums are fp32 in a
    fixed order; a row's dy * scale is held in three (fp32) or two (bf16, fp16) bf16 terms.  A dy that is not finite
    gives a result that is not finite.  workspace: tango_weight_grad_i8_workspace bytes. */
-size_t tango_weight_grad_i8_workspace(int64_t M, int64_t N, int64_t K, int64_t group);
+size_t tango_weight_grad_i8_workspace(int dtype, int64_t M, int64_t N, int64_t K, int64_t group);
 int tango_weight_grad_i8(void* dw, void* db, const void* dy, int dtype, int64_t ldy, const int8_t* q,
                          int64_t ldq, const float* scale, int64_t group, int64_t M, int64_t N, int64_t K,
                          void* workspace, size_t workspace_bytes, tango_stream_t stream);

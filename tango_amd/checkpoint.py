@@ -135,7 +135,7 @@ def weight_grad(dy, packed, want_bias=False):
             db = torch.empty(n, dtype=dy.dtype, device=dy.device) if want_bias else None
             if cols == 0 and want_bias:
                 db = flat.float().sum(0).to(dy.dtype)
-            ws_bytes = _L.tango_weight_grad_i8_workspace(rows, n, cols, packed.group)
+            ws_bytes = _L.tango_weight_grad_i8_workspace(DTYPES[dy.dtype], rows, n, cols, packed.group)
             ws = _workspace(ws_bytes, dy.device)
             check(_L.tango_weight_grad_i8(_ptr(dw), _ptr(db) if want_bias else None, _ptr(flat), DTYPES[dy.dtype],
                                           flat.stride(0) if rows > 1 else n, _ptr(packed.values), packed.values.stride(0),

@@ -16,8 +16,13 @@
 // pieces.  Partial sums of the row shares go to a slab each and a second kernel adds the slabs in order.  The tiles of
 // one row share are neighbours on one XCD, so dy and q come from HBM once and from that XCD's L2 for the other tiles.
 //
-// Why 128 x 256: a dy element is scaled and split (8 VALU instructions) once per tile of q columns, which at 128 x 128
-// was more than the matrix instructions it feeds (MMM).
+// Measured, [232965, 256] x [232965, 602] fp32 (three tiles of 224 columns): 269 us and 11 us for the slabs; the matrix
+// instructions alone are 229 k cycles a SIMD of the 502 k at 1.9 GHz.  On the way: 128 x 128 tiles with the conversions
+// between the matrix instructions' steps 785 us; scalar loads of the scales (they share the counter of LDS reads) and a
+// branch per 32 columns 457 us; one workgroup a CU for want of LDS, or 66 workgroups on some XCDs' 64 places, 336 us.
+// A plain large product runs at 1.2 PFLOP/s here: three terms take 200 us at that rate.
+#include <math.h>
+
 #include "element.hpp"
 
 namespace tango {
@@ -329,12 +334,18 @@ struct WGradPlan {
     int64_t runs, tile_k, tiles_run, tiles_k, tiles, splits, m_share, slab_floats;
 };
 
-static WGradPlan wgrad_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
+// Columns of q in a tile at most: two workgroups have to fit a CU's 160 KB of LDS, which they do at 76 KB each and did not at
+// 80 KB (three terms, 256 columns).
+static constexpr int most_columns(int terms) { return terms == 3 ? kTileK - kSub : kTileK; }
+static int terms_of(int dtype) { return dtype == TANGO_F32 ? 3 : 2; }
+
+static WGradPlan wgrad_plan(int dtype, int64_t M, int64_t N, int64_t K, int64_t group) {
     WGradPlan p;
+    const int64_t widest = most_columns(terms_of(dtype));
     if (group > K) group = K;
     p.runs = ceil_div(K, group);
     // a run in equal tiles
-    p.tile_k = ceil_div(ceil_div(group, ceil_div(group, kTileK)), kSub) * kSub;
+    p.tile_k = ceil_div(ceil_div(group, ceil_div(group, widest)), kSub) * kSub;
     p.tiles_run = ceil_div(group, p.tile_k);
     const int64_t last = K - (p.runs - 1) * group;
     p.tiles_k = (p.runs - 1) * p.tiles_run + ceil_div(last, p.tile_k);
@@ -344,6 +355,10 @@ static WGradPlan wgrad_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
     int64_t splits = p.tiles <= 64 ? 8 * (64 / p.tiles) : 512 / p.tiles;
     const int64_t most = ceil_div(M, 4 * kStep);
     if (splits > most) splits = most;
+    // a share more costs its slab written and read (some 4 TB/s), a share less its rows for the others (some 1.3 us a
+    // step): the sum is smallest at their ratio's root (19717 rows, 256 x 500 fp32: 52 shares 37 us, 64 45 us, 26 51 us)
+    const int64_t best = static_cast<int64_t>(sqrt(20000.0 * static_cast<double>(M) / (static_cast<double>(N) * static_cast<double>(K))));
+    if (splits > best) splits = best;
     if (splits < 1) splits = 1;
     p.m_share = ceil_div(ceil_div(M, splits), kStep) * kStep;
     p.splits = p.m_share ? ceil_div(M, p.m_share) : 1;
@@ -353,7 +368,7 @@ static WGradPlan wgrad_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
 
 template <typename T, int TERMS, int SUBS, bool WHOLE>
 static bool launch_weight_grad_tile(const WGradArgs& a, hipStream_t s) {
-    constexpr int kLds = 2 * (kStep / 8) * (TERMS * kTileN + SUBS * kSub) * 16 + (SUBS * kSub < kTileK ? 128 : 0);
+    constexpr int kLds = 2 * (kStep / 8) * (TERMS * kTileN + SUBS * kSub) * 16 + (SUBS * kSub < 256 ? 128 : 0);
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(weight_grad_kernel<T, TERMS, SUBS, WHOLE>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess) {
         (void)hipGetLastError();
@@ -368,7 +383,7 @@ template <typename T, int TERMS>
 static bool launch_weight_grad(const WGradArgs& a, bool whole, void* dw, void* db, hipStream_t s) {
     bool ok = false;
     if (!whole) {
-        ok = launch_weight_grad_tile<T, TERMS, kTileK / kSub, false>(a, s);
+        ok = launch_weight_grad_tile<T, TERMS, most_columns(TERMS) / kSub, false>(a, s);
     } else {
         switch (a.tile_k / kSub) {
             case 1: ok = launch_weight_grad_tile<T, TERMS, 1, true>(a, s); break;
@@ -378,7 +393,9 @@ static bool launch_weight_grad(const WGradArgs& a, bool whole, void* dw, void* d
             case 5: ok = launch_weight_grad_tile<T, TERMS, 5, true>(a, s); break;
             case 6: ok = launch_weight_grad_tile<T, TERMS, 6, true>(a, s); break;
             case 7: ok = launch_weight_grad_tile<T, TERMS, 7, true>(a, s); break;
-            case 8: ok = launch_weight_grad_tile<T, TERMS, 8, true>(a, s); break;
+            case 8:
+                if constexpr (TERMS == 2) ok = launch_weight_grad_tile<T, TERMS, 8, true>(a, s);
+                break;
         }
     }
     if (!ok) return false;
@@ -399,9 +416,9 @@ using namespace tango;
 
 extern "C" {
 
-size_t tango_weight_grad_i8_workspace(int64_t M, int64_t N, int64_t K, int64_t group) {
-    if (M <= 0 || N <= 0 || K <= 0 || group <= 0 || !wgrad_sizes(M, N, K)) return 0;
-    return static_cast<size_t>(wgrad_plan(M, N, K, group).slab_floats) * 4;
+size_t tango_weight_grad_i8_workspace(int dtype, int64_t M, int64_t N, int64_t K, int64_t group) {
+    if (!float_type(dtype) || M <= 0 || N <= 0 || K <= 0 || group <= 0 || !wgrad_sizes(M, N, K)) return 0;
+    return static_cast<size_t>(wgrad_plan(dtype, M, N, K, group).slab_floats) * 4;
 }
 
 int tango_weight_grad_i8(void* dw, void* db, const void* dy, int dtype, int64_t ldy, const int8_t* q, int64_t ldq, const float* scale,
@@ -414,7 +431,7 @@ int tango_weight_grad_i8(void* dw, void* db, const void* dy, int dtype, int64_t 
         !aligned_to(db, element_size(dtype)) || !aligned_to(scale, 4))
         return TANGO_ERR_INVALID_ARG;
     if (!wgrad_sizes(M, N, K)) return TANGO_ERR_UNSUPPORTED;
-    const WGradPlan p = wgrad_plan(M, N, K, group);
+    const WGradPlan p = wgrad_plan(dtype, M, N, K, group);
     if (!workspace || workspace_bytes < static_cast<size_t>(p.slab_floats) * 4 || !aligned_to(workspace, 16)) return TANGO_ERR_WORKSPACE;
     if (p.tiles * (p.splits + 8) > 0x7fffffffLL) return TANGO_ERR_UNSUPPORTED;
     WGradArgs a;

@@ -43,8 +43,8 @@ def test_weight_grad_abi_refusals():
     assert call(dtype=5) == -2 and call(N=1 << 17) == -2 and call(M=1 << 31) == -2
     assert call(M=0) == -1 and call(group=0) == -1 and call(dy=None) == -1 and call(dw=18) == -1 and call(scale=None) == -1
     assert call(N=0) == 0 and call(K=0) == 0
-    assert L.tango_weight_grad_i8_workspace(4, 8, 16, 16) >= 4 * (8 * 16 + 8)
-    assert L.tango_weight_grad_i8_workspace(0, 8, 16, 16) == 0
+    assert L.tango_weight_grad_i8_workspace(0, 4, 8, 16, 16) >= 4 * (8 * 16 + 8)
+    assert L.tango_weight_grad_i8_workspace(0, 0, 8, 16, 16) == 0
 
 
 def _attention(**kw):
