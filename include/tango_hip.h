@@ -602,8 +602,7 @@ int tango_batchnorm_bwd_f32(float* dx, float* dgamma, float* dbeta, const float*
    the last run of a row may be shorter, group >= cols gives one run a row.  Per run
      scale = max|x| / 127 (at most the largest whose 127-fold is finite),  q = the integer nearest to 127 x / max|x|, ties to even (decided exactly),
    and q * scale is the value held.  A run with an infinity or a NaN gets scale NaN and q = 0 (every value of it comes
-   back as NaN); a run of zeros gets scale 0.  The scale of (row, run) is at row * scale_row + run * scale_run.  Rows that start on
-   16-byte multiples and runs that are a multiple of 16 bytes take the widest loads; anything else is taken too. */
+   back as NaN); a run of zeros gets scale 0.  The scale of (row, run) is at row * scale_row + run * scale_run. */
 int tango_pack_i8(int8_t* q, int64_t ldq, float* scale, int64_t scale_row, int64_t scale_run, const void* x,
                   int dtype, int64_t rows, int64_t cols, int64_t ldx, int64_t group, tango_stream_t stream);
 /* x[r, c] = q[r, c] * scale[r, c / group] in fp32, then rounded to dtype.  scale: [rows, ceil(cols / group)]. */

@@ -44,44 +44,106 @@ __device__ __forceinline__ int nearest_127(float xs, float ts, float inv) {
 constexpr float kLargestScale = 0x1.0204060000000p+121f;
 
 struct RunScale {
-    float top, inv;  // scaled to [0.5, 1); 127 / top
-    int exp;
+    float top, inv, rec;  // the maximum scaled to [0.5, 1); 127 / top; 1 / top
+    float times;          // 127 times that power of two
     float scale;
+    int exp;
+    bool held, plain;     // finite and not zero; and in a range where nothing below over- or underflows
 };
 
 __device__ __forceinline__ RunScale run_scale(uint32_t top_bits) {
     RunScale r;
     const float top = __uint_as_float(top_bits);
-    if (top_bits >= 0x7f800000u) {
-        r.top = 1.0f;
-        r.inv = 0.0f;  // unused: the integers of such a run are 0
-        r.exp = 0;
-        r.scale = __uint_as_float(0x7fc00000u);
-    } else if (top_bits == 0) {
-        r.top = 1.0f;
-        r.inv = 127.0f;
-        r.exp = 0;
-        r.scale = 0.0f;
-    } else {
-        r.exp = __builtin_amdgcn_frexp_expf(top);
-        r.top = __builtin_amdgcn_ldexpf(top, -r.exp);
-        r.inv = 127.0f / r.top;
-        r.scale = fminf(top / 127.0f, kLargestScale);
-    }
+    r.held = top_bits != 0 && top_bits < 0x7f800000u;
+    r.exp = __builtin_amdgcn_frexp_expf(r.held ? top : 1.0f);
+    r.top = __builtin_amdgcn_ldexpf(r.held ? top : 1.0f, -r.exp);
+    r.inv = 127.0f / r.top;
+    r.rec = 1.0f / r.top;
+    r.plain = r.held && r.exp > -100 && r.exp < 100;
+    r.times = __builtin_amdgcn_ldexpf(127.0f, r.plain ? -r.exp : 0);
+    r.scale = r.held ? fminf(top / 127.0f, kLargestScale) : top_bits ? __uint_as_float(0x7fc00000u) : 0.0f;
     return r;
 }
 
 __device__ __forceinline__ int run_quant(float x, const RunScale& r) {
     const int n = nearest_127(__builtin_amdgcn_ldexpf(fabsf(x), -r.exp), r.top, r.inv);
-    return x < 0.0f ? -n : n;
+    return !r.held ? 0 : x < 0.0f ? -n : n;
 }
 
-// Maximum over `lanes` (a power of two) neighbouring lanes, in all of them.  Non-negative floats as their bits: a NaN
-// is the largest.
+// The integers of VEC elements, four to a word.  16-bit elements: 127 x is exact in fp32, and a quotient refined by one
+// step from a correctly rounded reciprocal is correctly rounded, so a tie, which is representable, is met exactly, and
+// nothing else in 16 bits comes within 2^-13 of one; six instructions an element.  fp32 elements: the approximate
+// quotient decides unless it is within 2^-14 of a tie (its error is below 2^-15); then nearest_127 does, for the whole
+// piece.  Either way what is far from the ordinary range goes to nearest_127.
+template <typename T, int VEC>
+__device__ __forceinline__ void quant_piece(const Pack<T, VEC>& in, const RunScale& r, int (&n)[VEC]) {
+    bool sure = r.plain;
+    if constexpr (sizeof(T) == 4) {
+        float far = 0.0f;
+        const float inv = __builtin_amdgcn_ldexpf(r.inv, r.plain ? -r.exp : 0);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float y = in.get(j) * inv, k = rintf(y);
+            far = fmaxf(far, fabsf(y - k));
+            n[j] = static_cast<int>(k);
+        }
+        sure = sure && far < 0.5f - 0x1p-14f;
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float t = in.get(j) * r.times, y0 = t * r.rec;
+            const float y = __builtin_fmaf(__builtin_fmaf(-y0, r.top, t), r.rec, y0);
+            n[j] = static_cast<int>(rintf(y));
+        }
+    }
+    if (!sure) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) n[j] = run_quant(in.get(j), r);
+    }
+}
+
+// The largest |x| of VEC elements as the bits of an fp32 number (ordered like the numbers; a NaN is the largest).
+template <typename T, int VEC, int R>
+__device__ __forceinline__ uint32_t largest_bits(const Pack<T, VEC> (&in)[R]) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    if constexpr (sizeof(T) == 4) {
+        uint32_t t = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) t = __builtin_elementwise_max(t, in[i].w[j] & 0x7fffffffu);
+        return t;
+    } else {
+        u16x2 t = {0, 0};
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < Pack<T, VEC>::kWords; ++j)
+                t = __builtin_elementwise_max(t, __builtin_bit_cast(u16x2, in[i].w[j] & 0x7fff7fffu));
+        const uint16_t most = t[0] > t[1] ? t[0] : t[1];
+        if constexpr (__is_same(T, bf16_t)) return static_cast<uint32_t>(most) << 16;
+        return __float_as_uint(static_cast<float>(__builtin_bit_cast(f16_t, most)));
+    }
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_umax(uint32_t v) {
+    return __builtin_elementwise_max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true)));
+}
+
+// Maximum over `lanes` (a power of two, the same for the whole launch) neighbouring lanes, in all of them.
 __device__ __forceinline__ uint32_t lanes_umax(uint32_t v, int lanes) {
-    for (int off = 1; off < lanes; off <<= 1) {
-        const uint32_t o = __shfl_xor(v, off, kWave);
-        v = o > v ? o : v;
+    if (lanes >= 2) v = dpp_umax<0xb1>(v);
+    if (lanes >= 4) v = dpp_umax<0x4e>(v);
+    if (lanes >= 8) v = dpp_umax<0x141>(v);
+    if (lanes >= 16) v = dpp_umax<0x140>(v);
+    if (lanes >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = __builtin_elementwise_max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
+    }
+    if (lanes >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = __builtin_elementwise_max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
     }
     return v;
 }
@@ -112,21 +174,18 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
             for (int i = 0; i < R; ++i) {
                 const int c = (i * a.lanes + lane) * VEC;
                 in[u][i].zero();
-                if (c < len[u]) in[u][i].load(src + c);
+                if constexpr (VEC == 1) {
+                    if (c < len[u]) in[u][i].load(src + c);
+                } else {
+                    if (c + VEC <= len[u])
+                        in[u][i].load_any(src + c);
+                    else if (c < len[u])
+                        in[u][i].load_some(src + c, len[u] - c);
+                }
             }
         }
 #pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            uint32_t t = 0;
-#pragma unroll
-            for (int i = 0; i < R; ++i)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const uint32_t b = __float_as_uint(in[u][i].get(j)) & 0x7fffffffu;
-                    t = b > t ? b : t;
-                }
-            top[u] = lanes_umax(t, a.lanes);
-        }
+        for (int u = 0; u < UN; ++u) top[u] = lanes_umax(largest_bits<T, VEC, R>(in[u]), a.lanes);
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
             if (!len[u]) continue;
@@ -138,12 +197,22 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
                 if (c >= len[u]) continue;
                 Pack<int8_t, VEC> o;
                 o.zero();
+                int n[VEC];
+                quant_piece<T, VEC>(in[u][i], r, n);
+                if constexpr (VEC == 1) {
+                    o.w[0] = static_cast<uint32_t>(n[0]) & 0xffu;
+                } else {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const int n = top[u] >= 0x7f800000u ? 0 : run_quant(in[u][i].get(j), r);
-                    o.w[j / 4] |= (static_cast<uint32_t>(n) & 0xffu) << (8 * (j & 3));
+                    for (int j = 0; j < VEC; j += 4) o.w[j / 4] = pack4(n[j], n[j + 1], n[j + 2], n[j + 3]);
                 }
-                o.store(dst + c);
+                if constexpr (VEC == 1) {
+                    o.store(dst + c);
+                } else {
+                    if (c + VEC <= len[u])
+                        o.store_any(dst + c);
+                    else
+                        o.store_some(dst + c, len[u] - c);
+                }
             }
             if (lane == 0) a.scale[row[u] * a.scale_row + run[u] * a.scale_run] = r.scale;
         }
@@ -174,7 +243,7 @@ __global__ __launch_bounds__(256) void pack_long_kernel(const PackArgs a) {
         const RunScale r = run_scale(t);
         int8_t* dst = a.q + row * a.ldq + col;
         for (int c = threadIdx.x; c < len; c += 256)
-            dst[c] = static_cast<int8_t>(t >= 0x7f800000u ? 0 : run_quant(widen(src[c]), r));
+            dst[c] = static_cast<int8_t>(run_quant(widen(src[c]), r));
         if (threadIdx.x == 0) a.scale[row * a.scale_row + (id - rw * a.groups.d) * a.scale_run] = r.scale;
     }
 }
@@ -184,9 +253,9 @@ struct UnpackArgs {
     const float* scale;
     void* x;
     int64_t ldx, ldq;
-    uint32_t total;  // pieces of VEC elements of this launch
-    int groups;
-    FastDiv per_row, per_group;  // pieces
+    uint32_t total;  // pieces of VEC elements of this launch; every run has as many, the last ones of a short run are empty
+    int cols, group;
+    FastDiv groups, per_run;
 };
 
 template <typename T, int VEC, int UN>
@@ -196,19 +265,32 @@ __global__ __launch_bounds__(256) void unpack_kernel(const UnpackArgs a) {
         Pack<int8_t, VEC> in[UN];
         float s[UN];
         int64_t to[UN];
+        int left[UN];
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
-            uint32_t id = first + u * stride;
-            id = id < a.total ? id : a.total - 1;
-            const uint32_t row = a.per_row.div(id);
-            const uint32_t piece = id - row * a.per_row.d;
-            in[u].load(a.q + static_cast<int64_t>(row) * a.ldq + piece * VEC);
-            s[u] = a.scale[static_cast<int64_t>(row) * a.groups + a.per_group.div(piece)];
-            to[u] = static_cast<int64_t>(row) * a.ldx + piece * VEC;
+            const bool ok = first + u * stride < a.total;
+            const uint32_t id = ok ? first + u * stride : 0;
+            const uint32_t run_id = a.per_run.div(id), row = a.groups.div(run_id);
+            const int run = static_cast<int>(run_id - row * a.groups.d), at = static_cast<int>(id - run_id * a.per_run.d) * VEC;
+            const int col = run * a.group + at;
+            const int end = a.cols - run * a.group < a.group ? a.cols - run * a.group : a.group;
+            left[u] = ok ? end - at : 0;
+            const int8_t* p = a.q + static_cast<int64_t>(row) * a.ldq + col;
+            in[u].zero();
+            if constexpr (VEC == 1) {
+                if (left[u] > 0) in[u].load(p);
+            } else {
+                if (left[u] >= VEC)
+                    in[u].load_any(p);
+                else if (left[u] > 0)
+                    in[u].load_some(p, left[u]);
+            }
+            s[u] = a.scale[run_id];
+            to[u] = static_cast<int64_t>(row) * a.ldx + col;
         }
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
-            if (first + u * stride >= a.total) continue;
+            if (left[u] <= 0) continue;
             float v[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
@@ -219,67 +301,73 @@ __global__ __launch_bounds__(256) void unpack_kernel(const UnpackArgs a) {
             }
             Pack<T, VEC> o;
             o.set_all(v);
-            o.store(static_cast<T*>(a.x) + to[u]);
+            T* p = static_cast<T*>(a.x) + to[u];
+            if constexpr (VEC == 1) {
+                o.store(p);
+            } else {
+                if (left[u] >= VEC)
+                    o.store_any(p);
+                else
+                    o.store_some(p, left[u]);
+            }
         }
     }
 }
 
-// The widest piece that every row start, run start and run end is a multiple of (the last run of a row ends at cols).
-static int piece_of(const void* x, int dtype, int64_t cols, int64_t ldx, int64_t group, const void* q, int64_t ldq) {
-    const int64_t size = element_size(dtype);
-    for (int vec = size == 4 ? 4 : 8; vec > 1; vec >>= 1) {
-        const bool runs = group >= cols || group % vec == 0;
-        if (runs && cols % vec == 0 && ldx % vec == 0 && ldq % vec == 0 && aligned_to(x, vec * size) && aligned_to(q, vec))
-            return vec;
-    }
-    return 1;
+// Pieces of 16 bytes of x at any alignment, the end of a run an element at a time; runs shorter than that altogether an
+// element at a time ([232965, 602] bf16, whose rows start on multiples of four bytes: 142 us with pieces of four bytes, PPP
+// with pieces of sixteen).
+static int piece_of(int dtype, int64_t cols, int64_t group) {
+    const int vec = dtype == TANGO_F32 ? 4 : 8;
+    return group >= vec && cols >= vec ? vec : 1;
+}
+
+template <typename T, int VEC, int R, int UN>
+static void launch_pack_pieces(const PackArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((pack_kernel<T, VEC, R, UN>), dim3(grid_for(ceil_div(a.total, UN), 256 / a.lanes)), dim3(256), 0, s, a);
 }
 
 template <typename T, int VEC>
 static void launch_pack_vec(PackArgs& a, hipStream_t s) {
     const int64_t run = a.group < a.cols ? a.group : a.cols;
     const int64_t pieces = ceil_div(run, VEC);
-    a.lanes = 1;
-    while (a.lanes < kWave && a.lanes < pieces) a.lanes <<= 1;
-    const int64_t per_lane = ceil_div(pieces, a.lanes);
-    const int blocks = grid_for(a.total, 256 / a.lanes);
-    if (per_lane <= 1)
-        hipLaunchKernelGGL((pack_kernel<T, VEC, 1, 4>), dim3(grid_for(ceil_div(a.total, 4), 256 / a.lanes)), dim3(256), 0, s, a);
-    else if (per_lane <= 2)
-        hipLaunchKernelGGL((pack_kernel<T, VEC, 2, 2>), dim3(grid_for(ceil_div(a.total, 2), 256 / a.lanes)), dim3(256), 0, s, a);
-    else if (per_lane <= 4)
-        hipLaunchKernelGGL((pack_kernel<T, VEC, 4, 1>), dim3(blocks), dim3(256), 0, s, a);
-    else if (per_lane <= 8)
-        hipLaunchKernelGGL((pack_kernel<T, VEC, 8, 1>), dim3(blocks), dim3(256), 0, s, a);
-    else if (per_lane <= 16)
-        hipLaunchKernelGGL((pack_kernel<T, VEC, 16, 1>), dim3(blocks), dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL((pack_long_kernel<T>), dim3(a.total < 2048 ? a.total : 2048), dim3(256), 0, s, a);
+    // lanes and pieces a lane with the fewest idle places (76 pieces: 16 lanes of 5, 64 lanes of 2 left 52 of 128 places
+    // idle and took 199 us where these take PPP), the more lanes the better among equals
+    int64_t best = 0, per_lane = 0;
+    for (int lanes = kWave; lanes >= 1; lanes >>= 1) {
+        const int64_t per = ceil_div(pieces, lanes);
+        if (per > 8 || (best && per * lanes >= best)) continue;
+        best = per * lanes;
+        per_lane = per;
+        a.lanes = lanes;
+    }
+    switch (per_lane) {
+        case 1: return launch_pack_pieces<T, VEC, 1, 4>(a, s);
+        case 2: return launch_pack_pieces<T, VEC, 2, 2>(a, s);
+        case 3: return launch_pack_pieces<T, VEC, 3, 2>(a, s);
+        case 4: return launch_pack_pieces<T, VEC, 4, 1>(a, s);
+        case 5: return launch_pack_pieces<T, VEC, 5, 1>(a, s);
+        case 6: return launch_pack_pieces<T, VEC, 6, 1>(a, s);
+        case 7: return launch_pack_pieces<T, VEC, 7, 1>(a, s);
+        case 8: return launch_pack_pieces<T, VEC, 8, 1>(a, s);
+    }
+    hipLaunchKernelGGL((pack_long_kernel<T>), dim3(a.total < 2048 ? a.total : 2048), dim3(256), 0, s, a);
 }
 
 template <typename T>
 static void launch_pack(PackArgs& a, int vec, hipStream_t s) {
-    if constexpr (sizeof(T) == 2) {
-        if (vec == 8) return launch_pack_vec<T, 8>(a, s);
-    }
-    if (vec == 4) return launch_pack_vec<T, 4>(a, s);
-    if (vec == 2) return launch_pack_vec<T, 2>(a, s);
-    launch_pack_vec<T, 1>(a, s);
-}
-
-template <typename T, int VEC>
-static void launch_unpack_vec(const UnpackArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL((unpack_kernel<T, VEC, 4>), dim3(grid_for(ceil_div(a.total, 4), 256)), dim3(256), 0, s, a);
+    constexpr int kWide = 16 / static_cast<int>(sizeof(T));
+    vec == 1 ? launch_pack_vec<T, 1>(a, s) : launch_pack_vec<T, kWide>(a, s);
 }
 
 template <typename T>
 static void launch_unpack(const UnpackArgs& a, int vec, hipStream_t s) {
-    if constexpr (sizeof(T) == 2) {
-        if (vec == 8) return launch_unpack_vec<T, 8>(a, s);
-    }
-    if (vec == 4) return launch_unpack_vec<T, 4>(a, s);
-    if (vec == 2) return launch_unpack_vec<T, 2>(a, s);
-    launch_unpack_vec<T, 1>(a, s);
+    constexpr int kWide = 16 / static_cast<int>(sizeof(T));
+    const dim3 grid(grid_for(ceil_div(a.total, 4), 256)), block(256);
+    if (vec == 1)
+        hipLaunchKernelGGL((unpack_kernel<T, 1, 4>), grid, block, 0, s, a);
+    else
+        hipLaunchKernelGGL((unpack_kernel<T, kWide, 4>), grid, block, 0, s, a);
 }
 
 static int check_pack(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int64_t group, const void* q,
@@ -307,7 +395,7 @@ int tango_pack_i8(int8_t* q, int64_t ldq, float* scale, int64_t scale_row, int64
     if (scale_row < 0 || scale_run < 0) return TANGO_ERR_INVALID_ARG;
     if (group > cols) group = cols;
     const int64_t groups = ceil_div(cols, group);
-    const int vec = piece_of(x, dtype, cols, ldx, group, q, ldq);
+    const int vec = piece_of(dtype, cols, group);
     const int64_t slab = ((1LL << 30) / groups) > 0 ? (1LL << 30) / groups : 1;  // runs of a launch stay below 2^31
     for (int64_t r0 = 0; r0 < rows; r0 += slab) {
         PackArgs a;
@@ -341,8 +429,8 @@ int tango_unpack_i8(void* x, int dtype, int64_t ldx, const int8_t* q, int64_t ld
     if (rows > 1 && ldx < cols) return TANGO_ERR_INVALID_ARG;
     if (group > cols) group = cols;
     const int64_t groups = ceil_div(cols, group);
-    const int vec = piece_of(x, dtype, cols, ldx, group, q, ldq);
-    const int64_t pieces = cols / vec;
+    const int vec = piece_of(dtype, cols, group);
+    const int64_t per_run = ceil_div(group, vec), pieces = groups * per_run;  // of a row
     const int64_t slab = ((1LL << 30) / pieces) > 0 ? (1LL << 30) / pieces : 1;
     for (int64_t r0 = 0; r0 < rows; r0 += slab) {
         const int64_t n = rows - r0 < slab ? rows - r0 : slab;
@@ -353,9 +441,10 @@ int tango_unpack_i8(void* x, int dtype, int64_t ldx, const int8_t* q, int64_t ld
         a.ldx = ldx;
         a.ldq = ldq;
         a.total = static_cast<uint32_t>(n * pieces);
-        a.groups = static_cast<int>(groups);
-        a.per_row = FastDiv(static_cast<uint32_t>(pieces));
-        a.per_group = FastDiv(static_cast<uint32_t>(group >= cols ? pieces : group / vec));
+        a.cols = static_cast<int>(cols);
+        a.group = static_cast<int>(group);
+        a.groups = FastDiv(static_cast<uint32_t>(groups));
+        a.per_run = FastDiv(static_cast<uint32_t>(per_run));
         if (dtype == TANGO_F32)
             launch_unpack<float>(a, vec, as_stream(stream));
         else if (dtype == TANGO_BF16)

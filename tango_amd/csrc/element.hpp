@@ -20,8 +20,11 @@ struct Pack {
     }
     // p at any multiple of an element: global memory takes vector accesses at any address
     __device__ __forceinline__ void load_any(const T* p) {
-        static_assert(kBytes == 8 || kBytes % 16 == 0, "whole vectors");
-        if constexpr (kBytes == 8) {
+        static_assert(kBytes == 4 || kBytes == 8 || kBytes % 16 == 0, "whole vectors");
+        if constexpr (kBytes == 4) {
+            typedef uint32_t U __attribute__((aligned(1)));
+            w[0] = *reinterpret_cast<const U*>(p);
+        } else if constexpr (kBytes == 8) {
             typedef u32x2 U __attribute__((aligned(1)));
             const u32x2 t = *reinterpret_cast<const U*>(p);
             w[0] = t[0];
@@ -37,15 +40,51 @@ struct Pack {
         }
     }
     __device__ __forceinline__ void store_any(T* p) const {
-        static_assert(kBytes % 16 == 0, "whole vectors");
-        typedef u32x4 U __attribute__((aligned(1)));
+        static_assert(kBytes == 4 || kBytes == 8 || kBytes % 16 == 0, "whole vectors");
+        if constexpr (kBytes == 4) {
+            typedef uint32_t U __attribute__((aligned(1)));
+            *reinterpret_cast<U*>(p) = w[0];
+        } else if constexpr (kBytes == 8) {
+            typedef u32x2 U __attribute__((aligned(1)));
+            u32x2 t;
+            t[0] = w[0];
+            t[1] = w[1];
+            *reinterpret_cast<U*>(p) = t;
+        } else {
+            typedef u32x4 U __attribute__((aligned(1)));
 #pragma unroll
-        for (int i = 0; i < kBytes / 16; ++i) {
-            u32x4 t;
+            for (int i = 0; i < kBytes / 16; ++i) {
+                u32x4 t;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) t[j] = w[4 * i + j];
-            reinterpret_cast<U*>(p)[i] = t;
+                for (int j = 0; j < 4; ++j) t[j] = w[4 * i + j];
+                reinterpret_cast<U*>(p)[i] = t;
+            }
         }
+    }
+    // The first n elements (n < VEC), the others zero; one access each.
+    __device__ __forceinline__ void load_some(const T* p, int n) {
+        constexpr int kBits = 8 * static_cast<int>(sizeof(T));
+        zero();
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (i < n) {
+                uint32_t one;
+                if constexpr (sizeof(T) == 4) one = *reinterpret_cast<const uint32_t*>(p + i);
+                if constexpr (sizeof(T) == 2) one = *reinterpret_cast<const uint16_t*>(p + i);
+                if constexpr (sizeof(T) == 1) one = *reinterpret_cast<const uint8_t*>(p + i);
+                w[i * kBits / 32] |= one << (i * kBits % 32);
+            }
+    }
+    __device__ __forceinline__ void store_some(T* p, int n) const {
+        constexpr int kBits = 8 * static_cast<int>(sizeof(T));
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (i < n) {
+                const uint32_t one = w[i * kBits / 32] >> (i * kBits % 32);
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(p + i) = one;
+                if constexpr (sizeof(T) == 2) *reinterpret_cast<uint16_t*>(p + i) = static_cast<uint16_t>(one);
+                if constexpr (sizeof(T) == 1) *reinterpret_cast<uint8_t*>(p + i) = static_cast<uint8_t>(one);
+            }
     }
     // p aligned to min(kBytes, 16)
     __device__ __forceinline__ void load(const T* p) {
