@@ -314,12 +314,14 @@ __global__ __launch_bounds__(256) void unpack_kernel(const UnpackArgs a) {
     }
 }
 
-// Pieces of 16 bytes of x at any alignment, the end of a run an element at a time; runs shorter than that altogether an
-// element at a time ([232965, 602] bf16, whose rows start on multiples of four bytes: 142 us with pieces of four bytes, PPP
-// with pieces of sixteen).
-static int piece_of(int dtype, int64_t cols, int64_t group) {
-    const int vec = dtype == TANGO_F32 ? 4 : 8;
-    return group >= vec && cols >= vec ? vec : 1;
+// Elements of a piece, at any alignment, the end of a run an element at a time; runs shorter than a piece altogether so.
+// 16-bit types: 16 bytes ([232965, 602] bf16, whose rows start on multiples of four bytes: packed in 109 us, 142 us with
+// pieces of four bytes).  fp32: 16 bytes restored, 32 packed where a run has them, so that 8 bytes are stored
+// ([169343, 256] in runs of 32: 56 us against 59 us; restored with 32 bytes 37 us against 35 us).
+static int piece_of(int dtype, int64_t cols, int64_t group, bool packing) {
+    const int64_t run = group < cols ? group : cols;
+    if (run >= 8 && (dtype != TANGO_F32 || packing)) return 8;
+    return run >= 4 && dtype == TANGO_F32 ? 4 : 1;
 }
 
 template <typename T, int VEC, int R, int UN>
@@ -331,8 +333,8 @@ template <typename T, int VEC>
 static void launch_pack_vec(PackArgs& a, hipStream_t s) {
     const int64_t run = a.group < a.cols ? a.group : a.cols;
     const int64_t pieces = ceil_div(run, VEC);
-    // lanes and pieces a lane with the fewest idle places (76 pieces: 16 lanes of 5, 64 lanes of 2 left 52 of 128 places
-    // idle and took 199 us where these take PPP), the more lanes the better among equals
+    // lanes and pieces a lane with the fewest idle places (76 pieces: 16 lanes of 5; 64 lanes of 2 leave 52 of 128
+    // places idle), the more lanes the better among equals
     int64_t best = 0, per_lane = 0;
     for (int lanes = kWave; lanes >= 1; lanes >>= 1) {
         const int64_t per = ceil_div(pieces, lanes);
@@ -356,8 +358,11 @@ static void launch_pack_vec(PackArgs& a, hipStream_t s) {
 
 template <typename T>
 static void launch_pack(PackArgs& a, int vec, hipStream_t s) {
-    constexpr int kWide = 16 / static_cast<int>(sizeof(T));
-    vec == 1 ? launch_pack_vec<T, 1>(a, s) : launch_pack_vec<T, kWide>(a, s);
+    if (vec == 8) return launch_pack_vec<T, 8>(a, s);
+    if constexpr (sizeof(T) == 4) {
+        if (vec == 4) return launch_pack_vec<T, 4>(a, s);
+    }
+    launch_pack_vec<T, 1>(a, s);
 }
 
 template <typename T>
@@ -395,7 +400,7 @@ int tango_pack_i8(int8_t* q, int64_t ldq, float* scale, int64_t scale_row, int64
     if (scale_row < 0 || scale_run < 0) return TANGO_ERR_INVALID_ARG;
     if (group > cols) group = cols;
     const int64_t groups = ceil_div(cols, group);
-    const int vec = piece_of(dtype, cols, group);
+    const int vec = piece_of(dtype, cols, group, true);
     const int64_t slab = ((1LL << 30) / groups) > 0 ? (1LL << 30) / groups : 1;  // runs of a launch stay below 2^31
     for (int64_t r0 = 0; r0 < rows; r0 += slab) {
         PackArgs a;
@@ -429,7 +434,7 @@ int tango_unpack_i8(void* x, int dtype, int64_t ldx, const int8_t* q, int64_t ld
     if (rows > 1 && ldx < cols) return TANGO_ERR_INVALID_ARG;
     if (group > cols) group = cols;
     const int64_t groups = ceil_div(cols, group);
-    const int vec = piece_of(dtype, cols, group);
+    const int vec = piece_of(dtype, cols, group, false);
     const int64_t per_run = ceil_div(group, vec), pieces = groups * per_run;  // of a row
     const int64_t slab = ((1LL << 30) / pieces) > 0 ? (1LL << 30) / pieces : 1;
     for (int64_t r0 = 0; r0 < rows; r0 += slab) {
