@@ -27,27 +27,37 @@ def item_edges(edges):
     return cap
 
 
+# Rows up to which the items are computed on the host: some thirty small operations and three counts read back take
+# the device about half a millisecond whatever the size, the host that long from some ten thousand rows on.
+HOST_ROWS = 8192
+
+
 class AttentionItems:
     """One orientation of a graph cut into work items (``tango_attn_items`` of include/tango_hip.h)."""
 
     def __init__(self, indptr, indices, edge_ids, cap=None):
         cap = item_edges(indices.numel()) if cap is None else cap
+        device = indptr.device
+        rows = indptr.numel() - 1
+        if rows <= HOST_ROWS:
+            indptr = indptr.cpu()
         dev = indptr.device
-        degree = indptr[1:] - indptr[:-1]
-        rows = degree.numel()
-        pieces = torch.clamp((degree + cap - 1) // cap, min=1)
+        first_slot, last_slot = indptr[:-1], indptr[1:]
+        degree = last_slot - first_slot
+        pieces = torch.clamp((degree + (cap - 1)) // cap, min=1)
         row = torch.repeat_interleave(torch.arange(rows, device=dev), pieces)
         nth = torch.arange(row.numel(), device=dev) - (torch.cumsum(pieces, 0) - pieces)[row]
         size = ((degree + pieces - 1) // pieces)[row]
-        first = indptr[row] + nth * size
-        last = torch.minimum(first + size, indptr[1:][row])
+        first = first_slot[row] + nth * size
+        last = torch.minimum(first + size, last_slot[row])
         cut = pieces[row] > 1
         part = torch.where(cut, torch.cumsum(cut, 0) - 1, -1)
         order = torch.sort(last - first, descending=True, stable=True).indices
-        self.items = torch.stack([row, first, last, part], 1)[order].to(torch.int32).contiguous()
+        items = torch.stack([row, first, last, part], 1)[order].to(torch.int32)
         split = torch.nonzero(pieces > 1).flatten()
         ends = torch.cumsum(pieces[split], 0)
-        self.split = torch.stack([split, ends - pieces[split], ends, torch.zeros_like(split)], 1).to(torch.int32).contiguous()
+        split_items = torch.stack([split, ends - pieces[split], ends, torch.zeros_like(split)], 1).to(torch.int32)
+        self.items, self.split = items.to(device).contiguous(), split_items.to(device).contiguous()
         self.indices, self.edge_ids = indices, edge_ids
         s = _lib.AttnItems()
         s.num_items, s.num_split, s.num_edges = self.items.size(0), self.split.size(0), indices.numel()
@@ -85,20 +95,7 @@ def prepare_attention(graph):
 
 
 def _unit_last(t):
-    return t if t.dim() == 0 or t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
-
-
-def _struct(q_shape, k_shape, scale, dtype):
-    t = _lib.Attention()
-    t.num_dst, t.heads, t.dim = q_shape
-    t.num_src, t.kv_heads = k_shape[:2]
-    t.dtype, t.scale = DTYPES[dtype], scale
-    return t
-
-
-def _operands(t, q, k, v):
-    t.q, t.k, t.v = _ptr(q), _ptr(k), _ptr(v)
-    (t.q_row, t.q_head), (t.k_row, t.k_head), (t.v_row, t.v_head) = (x.stride()[:2] for x in (q, k, v))
+    return t if t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
 def _hold(q, k, v):
@@ -111,16 +108,23 @@ def _hold(q, k, v):
     return held, scales
 
 
-def _checkpoint_operands(t, held, scales):
-    t.checkpoint = 1
-    for name, x in zip("qkv", held):
-        setattr(t, name, _ptr(x))
-        setattr(t, name + "_row", x.stride(0))
-        setattr(t, name + "_head", t.dim)
-    t.q_scale_row, t.q_scale_head = scales[0].stride()[:2]
-    t.kv_scale_row, t.kv_scale_head = scales[1].stride()[:2]
-    t.q_scale, t.k_scale = _ptr(scales[0]), _ptr(scales[1])
-    t.v_scale = t.k_scale + 4 if t.k_scale else None
+def _struct(q, k, v, scale):
+    """tango_attention of the tensors themselves."""
+    n, heads, dim = q.shape
+    (qr, qh, _), (kr, kh, _), (vr, vh, _) = q.stride(), k.stride(), v.stride()
+    return _lib.Attention(n, k.size(0), heads, k.size(1), dim, DTYPES[q.dtype], 0, _ptr(q), _ptr(k), _ptr(v), qr, qh, kr, kh, vr, vh,
+                          None, None, None, 0, 0, 0, 0, scale)
+
+
+def _struct_held(q_shape, k_shape, dtype, held, scales, scale):
+    """tango_attention of their 8-bit forms."""
+    (n, heads, dim), (m, kv_heads, _) = q_shape, k_shape
+    q, k, v = held
+    q_scale, kv_scale = scales
+    at = _ptr(kv_scale)
+    return _lib.Attention(n, m, heads, kv_heads, dim, DTYPES[dtype], 1, _ptr(q), _ptr(k), _ptr(v), q.stride(0), dim, k.stride(0), dim,
+                          v.stride(0), dim, _ptr(q_scale), at, at + 4 if at else None, *q_scale.stride()[:2],
+                          *kv_scale.stride()[:2], scale)
 
 
 class _GraphAttention(Function):
@@ -130,9 +134,7 @@ class _GraphAttention(Function):
             by_dst = _items(graph, "in")
             q, k, v = _unit_last(q), _unit_last(k), _unit_last(v)
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            t = _struct(q.shape, k.shape, scale, q.dtype)
-            _operands(t, q, k, v)
-            ref = ctypes.byref(t)
+            ref = ctypes.byref(_struct(q, k, v, scale))
             ws_bytes = _L.tango_graph_attention_workspace(ref, by_dst.ref, None, edge_mask is not None)
             ws = _workspace(ws_bytes, q.device)
             check(_L.tango_graph_attention_fwd(_ptr(out), ref, by_dst.ref, _ptr(edge_mask), _ptr(ws), ws_bytes, _stream()),
@@ -156,21 +158,19 @@ class _GraphAttention(Function):
             edge_mask, *qkv = ctx.saved_tensors
             dout = _unit_last(dout)
             if ctx.held is None:
+                t = _struct(*qkv, ctx.scale)
                 q_shape, k_shape = qkv[0].shape, qkv[1].shape
-                t = _struct(q_shape, k_shape, ctx.scale, qkv[0].dtype)
-                _operands(t, *qkv)
             else:
                 q_shape, k_shape, dtype = ctx.shapes
-                t = _struct(q_shape, k_shape, ctx.scale, dtype)
-                _checkpoint_operands(t, *ctx.held)
+                t = _struct_held(q_shape, k_shape, dtype, *ctx.held, ctx.scale)
             grads = [torch.empty(shape, dtype=dout.dtype, device=dout.device) if need else None
                      for shape, need in zip((q_shape, k_shape, k_shape), ctx.needs_input_grad[1:4])]
             ref = ctypes.byref(t)
             ws_bytes = _L.tango_graph_attention_workspace(ref, by_dst.ref, by_src.ref, edge_mask is not None)
             ws = _workspace(ws_bytes, dout.device)
-            check(_L.tango_graph_attention_bwd(*(None if g is None else _ptr(g) for g in grads), ref, _ptr(dout),
-                                               dout.stride(0), dout.stride(1), by_dst.ref, by_src.ref, _ptr(edge_mask),
-                                               _ptr(ws), ws_bytes, _stream()), "graph_attention.backward")
+            check(_L.tango_graph_attention_bwd(*map(_ptr, grads), ref, _ptr(dout), dout.stride(0), dout.stride(1), by_dst.ref,
+                                               by_src.ref, _ptr(edge_mask), _ptr(ws), ws_bytes, _stream()),
+                  "graph_attention.backward")
         return None, grads[0], grads[1], grads[2], None, None, None
 
 
@@ -189,20 +189,22 @@ def graph_attention(graph, q, k, v, scale=None, edge_mask=None, checkpoint=None)
         need_float(t, name)
         if t.dim() != 3:
             raise RuntimeError("graph_attention: %s must be [nodes, heads, dim]" % name)
-        if t.dtype != q.dtype or t.device != q.device:
-            raise RuntimeError("graph_attention: q, k and v must have one type and one device")
+    if not (q.dtype == k.dtype == v.dtype and q.device == k.device == v.device):
+        raise RuntimeError("graph_attention: q, k and v must have one type and one device")
     if not hasattr(graph, "adj_csc32"):
         raise RuntimeError("graph_attention: the graph has not been through graph_preprocess")
-    num_dst, num_src = graph.adj_csc[0].numel() - 1, graph.adj_csr[0].numel() - 1
-    if q.size(0) != num_dst or k.size(0) != num_src:
+    by_dst = graph.adj_csc[0]
+    num_dst, num_src = by_dst.size(0) - 1, graph.adj_csr[0].size(0) - 1
+    (rows, heads, dim), (k_rows, kv_heads, k_dim) = q.shape, k.shape
+    if rows != num_dst or k_rows != num_src:
         raise RuntimeError("graph_attention: q needs a row per destination (%d), k and v one per source (%d)" % (num_dst, num_src))
-    if k.shape != v.shape or q.size(2) != k.size(2):
+    if k.shape != v.shape or k_dim != dim:
         raise RuntimeError("graph_attention: k and v must have one shape, and q their dim")
-    if not 1 <= q.size(2) <= 256:
+    if not 1 <= dim <= 256:
         raise ValueError("graph_attention: dim must be 1 .. 256")
-    if k.size(1) < 1 or q.size(1) % k.size(1) or q.size(1) < 1:
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError("graph_attention: heads must be a multiple of kv_heads")
-    if graph.adj_csc[0].device != q.device:
+    if by_dst.device != q.device:
         raise RuntimeError("graph_attention: the graph and the tensors must be on one device")
     if edge_mask is not None:
         if not isinstance(edge_mask, torch.Tensor) or edge_mask.dtype != torch.bool or edge_mask.device != q.device:
@@ -212,7 +214,7 @@ def graph_attention(graph, q, k, v, scale=None, edge_mask=None, checkpoint=None)
         edge_mask = edge_mask.contiguous()
     if checkpoint not in (None, "int8"):
         raise ValueError("graph_attention: checkpoint must be None or 'int8'")
-    scale = 1.0 / math.sqrt(q.size(2)) if scale is None else float(scale)
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError("graph_attention: scale must be finite")
     return _GraphAttention.apply(graph, q, k, v, scale, edge_mask, checkpoint == "int8")
