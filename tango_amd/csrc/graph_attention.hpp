@@ -210,11 +210,16 @@ __device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.0
 // log2 of the softmax's denominator; +inf for a destination that nothing is left of, so that 2^(logit - it) is 0
 __device__ __forceinline__ float log2_total(float m, float l) { return l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l); }
 
-constexpr int kEdgesInFlight = 4;
+// Edges of a step (rows of both gathered tensors are in flight together; more cost registers and so wavefronts).
+// Forward at 2 / 4 / 6 / 8: 424 / 413 / 391 / 387 us ([169343, 8, 32] fp32, 1.3 M edges), 577 / 552 / 553 / 605 us (5.3 M
+// edges, heads 8 over 2).  dq: 456 / 430 / 425 / 422 us, from checkpoints [169343, 4, 64] 197 / 225 / 235 / 213 us;
+// dk, dv: 489 / 486 / 492 / 541 us, from checkpoints 310 / 315 / 351 / 532 us.
+constexpr int kForwardEdges = 6;
+constexpr int backward_edges(bool scaled) { return scaled ? 2 : 4; }
 
 template <typename T, int VEC, int LPH, int MODE>
 __global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnArgs a) {
-    constexpr int U = kEdgesInFlight;
+    constexpr int U = kForwardEdges;
     const ItemLane L = item_lane<LPH>(a, a.heads);
     if (!L.on) return;
     const RowLane<VEC, LPH, MODE> lane(L.j, a.dim);
@@ -329,8 +334,8 @@ struct AttnStat {
 // T: what q, k, v are held in (int8_t: checkpoints, with a scale per row and head); TG: dout and the results
 template <typename T, typename TG, int VEC, int LPH, int MODE>
 __global__ __launch_bounds__(256) void attn_bwd_q_kernel(const AttnArgs a) {
-    constexpr int U = kEdgesInFlight;
     typedef RowScale<T> S;
+    constexpr int U = backward_edges(S::kScaled);
     const ItemLane L = item_lane<LPH>(a, a.heads);
     if (!L.on) return;
     const RowLane<VEC, LPH, MODE> lane(L.j, a.dim);
@@ -444,8 +449,8 @@ __global__ __launch_bounds__(256) void attn_bwd_q_kernel(const AttnArgs a) {
 
 template <typename T, typename TG, int VEC, int LPH, int MODE>
 __global__ __launch_bounds__(256) void attn_bwd_kv_kernel(const AttnArgs a) {
-    constexpr int U = kEdgesInFlight;
     typedef RowScale<T> S;
+    constexpr int U = backward_edges(S::kScaled);
     const ItemLane L = item_lane<LPH>(a, a.kv_heads);
     if (!L.on) return;
     const RowLane<VEC, LPH, MODE> lane(L.j, a.dim);
