@@ -612,7 +612,7 @@ int tango_unpack_i8(void* x, int dtype, int64_t ldx, const int8_t* q, int64_t ld
 /* Gradients of a linear layer's weight and bias from the 8-bit checkpoint of its input (q [M, ldq], scale [M, runs] and
    group as of tango_pack_i8; every row of q is readable to ldq.  ldq, group and q multiples of 4 are the fast case):
      dw[n, k] = sum_m dy[m, n] * (q[m, k] * scale[m, k / group]),   db[n] = sum_m dy[m, n]  (db may be NULL)
-   for dy [M, N] (dtype, row stride ldy) and q [M, K]; dw [N, K] and db [N] in dtype, contiguous.  Sums are fp32 in a
+   for dy [M, N] (dtype, row stride ldy) and q [M, K], M <= 2^30, N and K <= 65536; dw [N, K] and db [N] in dtype, contiguous.  Sums are fp32 in a
    fixed order; a row's dy * scale is held in three (fp32) or two (bf16, fp16) bf16 terms.  A dy that is not finite
    gives a result that is not finite.  workspace: tango_weight_grad_i8_workspace bytes. */
 size_t tango_weight_grad_i8_workspace(int dtype, int64_t M, int64_t N, int64_t K, int64_t group);
@@ -637,7 +637,7 @@ typedef struct tango_attention {
 
 /* The rows of one orientation (destinations with their in-edges, or sources with their out-edges) as work items. */
 typedef struct tango_attn_items {
-    int64_t num_items, num_parts, num_split, num_edges;
+    int64_t num_items, num_parts, num_split, num_edges; /* num_edges <= 2^30 */
     const int32_t* items;    /* [num_items, 4]: row, first slot, last slot + 1, part or -1.  Every row is one item (part
                                 -1) or several, whose parts are consecutive and in slot order; 16-byte aligned */
     const int32_t* split;    /* [num_split, 4]: a row of several items, its first part, its last part + 1, 0 */

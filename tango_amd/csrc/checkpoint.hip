@@ -72,7 +72,7 @@ __device__ __forceinline__ int run_quant(float x, const RunScale& r) {
 
 // The integers of VEC elements, four to a word.  16-bit elements: 127 x is exact in fp32, and a quotient refined by one
 // step from a correctly rounded reciprocal is correctly rounded, so a tie, which is representable, is met exactly, and
-// nothing else in 16 bits comes within 2^-13 of one; six instructions an element.  fp32 elements: the approximate
+// no other quotient of 16-bit numbers (11 bits at most) is closer to one than 2^-19 of itself; six instructions an element.  fp32 elements: the approximate
 // quotient decides unless it is within 2^-14 of a tie (its error is below 2^-15); then nearest_127 does, for the whole
 // piece.  Either way what is far from the ordinary range goes to nearest_127.
 template <typename T, int VEC>

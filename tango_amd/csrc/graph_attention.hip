@@ -34,7 +34,7 @@ static int check_shape(const tango_attention* t) {
 
 static int check_items(const tango_attn_items* i, int64_t rows) {
     if (!i || i->num_items < 0 || i->num_parts < 0 || i->num_split < 0 || i->num_edges < 0) return TANGO_ERR_INVALID_ARG;
-    if (i->num_edges > (1LL << 31) - 4096 || i->num_parts >= (1LL << 31)) return TANGO_ERR_UNSUPPORTED;
+    if (i->num_edges > (1LL << 30) || i->num_parts >= (1LL << 31)) return TANGO_ERR_UNSUPPORTED;
     if (i->num_items < rows || i->num_split > i->num_parts) return TANGO_ERR_INVALID_ARG;  // every row is at least one item
     if ((i->num_items && (!i->items || !aligned_to(i->items, 16))) || (i->num_split && (!i->split || !aligned_to(i->split, 16))))
         return TANGO_ERR_INVALID_ARG;

@@ -622,10 +622,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const JoinArgs a) {
 static __global__ __launch_bounds__(256) void attn_mask_kernel(int32_t* out, const int32_t* indices, const int32_t* edge_ids,
                                                                const uint8_t* mask, uint32_t n) {
     const uint32_t stride = gridDim.x * 256;
-    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
-        const bool kept = mask[edge_ids ? static_cast<uint32_t>(edge_ids[i]) : i];
-        out[i] = kept ? indices[i] : -1;
-    }
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += stride)
+        out[i] = mask[edge_ids ? static_cast<uint32_t>(edge_ids[i]) : i] ? indices[i] : -1;
 }
 
 enum AttnPass { kPassForward, kPassQuery, kPassKeyValue };

@@ -407,7 +407,7 @@ static bool launch_weight_grad(const WGradArgs& a, bool whole, void* dw, void* d
 
 // sizes whose tile counts and offsets into a slab stay within the kernels' 32-bit numbers
 static bool wgrad_sizes(int64_t M, int64_t N, int64_t K) {
-    return M < (1LL << 31) && N <= 65536 && K <= 65536;
+    return M <= (1LL << 30) && N <= 65536 && K <= 65536;
 }
 
 }  // namespace tango
