@@ -311,23 +311,31 @@ __global__ __launch_bounds__(256, 2) void weight_grad_kernel(const WGradArgs a) 
     }
 }
 
-// Adds the row shares' slabs in order; the last workgroups do the bias.
+// Adds the row shares' slabs: a workgroup owns 32 results, its eight groups of 32 lanes take every eighth slab, their sums
+// are added in order (one lane for all slabs of a result: 50 us of the 65 for 482 slabs of [40, 128]).  Results past the
+// weight's are the bias's.
 template <typename T>
 __global__ __launch_bounds__(256) void weight_grad_sum_kernel(T* dw, T* db, const float* slab, const float* slab_b, int64_t count,
                                                               int n, int splits) {
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const bool bias = id >= count;
-    const float* p = bias ? slab_b : slab;
-    const int64_t at = bias ? id - count : id, step = bias ? n : count;
-    if (bias && (!db || at >= n)) return;
+    __shared__ float part[8][32];
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+    const bool bias = id >= count, on = id < count + (db ? n : 0);
+    const float* p = bias ? slab_b + (id - count) : slab + id;
+    const int64_t step = bias ? n : count;
     float t = 0.0f;
-    int s = 0;
-    for (; s + 4 <= splits; s += 4) {
-        const float x0 = p[s * step + at], x1 = p[(s + 1) * step + at], x2 = p[(s + 2) * step + at], x3 = p[(s + 3) * step + at];
-        t = (((t + x0) + x1) + x2) + x3;
+    if (on) {
+#pragma unroll 4
+        for (int s = slice; s < splits; s += 8) t += p[s * step];
     }
-    for (; s < splits; ++s) t += p[s * step + at];
-    (bias ? db : dw)[at] = static_cast<T>(t);
+    part[slice][lane] = t;
+    __syncthreads();
+    if (slice || !on) return;
+    for (int s = 1; s < 8; ++s) t += part[s][lane];
+    if (bias)
+        db[id - count] = static_cast<T>(t);
+    else
+        dw[id] = static_cast<T>(t);
 }
 
 struct WGradPlan {
@@ -400,7 +408,7 @@ static bool launch_weight_grad(const WGradArgs& a, bool whole, void* dw, void* d
     }
     if (!ok) return false;
     const int64_t count = static_cast<int64_t>(a.N) * a.K;
-    hipLaunchKernelGGL((weight_grad_sum_kernel<T>), dim3(static_cast<uint32_t>(ceil_div(count + (db ? a.N : 0), 256))), dim3(256), 0, s,
+    hipLaunchKernelGGL((weight_grad_sum_kernel<T>), dim3(static_cast<uint32_t>(ceil_div(count + (db ? a.N : 0), 32))), dim3(256), 0, s,
                        static_cast<T*>(dw), static_cast<T*>(db), a.slab, a.slab_b, count, a.N, a.splits);
     return true;
 }
