@@ -645,6 +645,13 @@ typedef struct tango_attn_items {
     const int32_t* edge_ids; /* [num_edges] or NULL (a slot's number is its edge's id): what edge_mask is indexed by */
 } tango_attn_items;
 
+/* Fills items and split for the rows of `indptr` [rows + 1] (their degrees sum up to num_edges), no item longer than cap
+   (1 .. 512), longest first.  items: room for rows + num_edges / cap entries of four, split: for num_edges / cap.
+   counts: tango_attention_items_workspace() bytes of device memory that hold zeros; its first two int32 then are
+   num_split and num_parts, and num_items = rows - num_split + num_parts. */
+size_t tango_attention_items_workspace(void);
+int tango_attention_items(int32_t* items, int32_t* split, const int64_t* indptr, int64_t rows, int64_t num_edges,
+                          int64_t cap, void* counts, size_t counts_bytes, tango_stream_t stream);
 /* Bytes of scratch for the forward pass (by_src NULL) or the backward pass; masked: a call with an edge_mask. */
 size_t tango_graph_attention_workspace(const tango_attention* t, const tango_attn_items* by_dst,
                                        const tango_attn_items* by_src, int masked);

@@ -81,6 +81,8 @@ SIGNATURES = {
     "tango_unpack_i8": (I, [P, I, I64, P, I64, P, I64, I64, I64, P]),
     "tango_weight_grad_i8_workspace": (SZ, [I, I64, I64, I64, I64]),
     "tango_weight_grad_i8": (I, [P, P, P, I, I64, P, I64, P, I64, I64, I64, I64, P, SZ, P]),
+    "tango_attention_items_workspace": (SZ, []),
+    "tango_attention_items": (I, [P, P, P, I64, I64, I64, P, SZ, P]),
     "tango_graph_attention_workspace": (SZ, [P, P, P, I]),
     "tango_graph_attention_fwd": (I, [P, P, P, P, P, SZ, P]),
     "tango_graph_attention_bwd": (I, [P, P, P, P, P, I64, I64, P, P, P, P, SZ, P]),

@@ -142,11 +142,115 @@ static void use_items(AttnArgs& a, JoinArgs& j, const tango_attn_items& i, const
     j.scale = a.scale;
 }
 
+// ---- Work items.  A row of d edges is ceil(d / cap) pieces (one if d is 0) of ceil(d / pieces) edges, the last one
+// shorter; items are counted by length, the counts become the first places of the lengths, longest first, and the pieces
+// take places.  Which of equal lengths comes first depends on the order of the workgroups, what is computed from the
+// items does not: an item owns its row or a numbered part of it.
+
+constexpr int kLengths = 513;  // 0 .. 512 edges
+
+struct ItemCounts {
+    int32_t split, parts;
+    int32_t place[kLengths];  // items of a length, then the next place of one
+};
+
+struct RowPieces {
+    int64_t first;
+    int degree, pieces, size, last;  // pieces - 1 of `size` edges and one of `last`
+};
+
+__device__ __forceinline__ RowPieces row_pieces(const int64_t* indptr, int64_t row, int cap) {
+    RowPieces p;
+    p.first = indptr[row];
+    p.degree = static_cast<int>(indptr[row + 1] - p.first);
+    p.pieces = p.degree > cap ? (p.degree + cap - 1) / cap : 1;
+    p.size = (p.degree + p.pieces - 1) / p.pieces;
+    p.last = p.degree - (p.pieces - 1) * p.size;
+    return p;
+}
+
+static __global__ __launch_bounds__(256) void items_count_kernel(ItemCounts* c, const int64_t* indptr, int64_t rows, int cap) {
+    __shared__ int32_t count[kLengths];
+    for (int i = threadIdx.x; i < kLengths; i += 256) count[i] = 0;
+    __syncthreads();
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (row < rows) {
+        const RowPieces p = row_pieces(indptr, row, cap);
+        if (p.pieces > 1) atomicAdd(&count[p.size], p.pieces - 1);
+        atomicAdd(&count[p.last], 1);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kLengths; i += 256)
+        if (count[i]) atomicAdd(&c->place[i], count[i]);
+}
+
+static __global__ __launch_bounds__(64) void items_scan_kernel(ItemCounts* c) {
+    if (threadIdx.x) return;
+    int32_t at = 0;
+    for (int i = kLengths - 1; i >= 0; --i) {
+        const int32_t n = c->place[i];
+        c->place[i] = at;
+        at += n;
+    }
+}
+
+static __global__ __launch_bounds__(256) void items_place_kernel(int4* items, int4* split, ItemCounts* c, const int64_t* indptr,
+                                                                 int64_t rows, int cap) {
+    __shared__ int32_t count[kLengths], base[kLengths];
+    for (int i = threadIdx.x; i < kLengths; i += 256) count[i] = 0;
+    __syncthreads();
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const bool on = row < rows;
+    RowPieces p = {0, 0, 1, 0, 0};
+    int32_t full_at = 0, last_at = 0;
+    if (on) {
+        p = row_pieces(indptr, row, cap);
+        if (p.pieces > 1) full_at = atomicAdd(&count[p.size], p.pieces - 1);
+        last_at = atomicAdd(&count[p.last], 1);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kLengths; i += 256)
+        if (count[i]) base[i] = atomicAdd(&c->place[i], count[i]);
+    __syncthreads();
+    if (!on) return;
+    const int r = static_cast<int>(row), first = static_cast<int>(p.first);
+    int part = -1;
+    if (p.pieces > 1) {
+        part = atomicAdd(&c->parts, p.pieces);
+        split[atomicAdd(&c->split, 1)] = make_int4(r, part, part + p.pieces, 0);
+        full_at += base[p.size];
+        for (int i = 0; i + 1 < p.pieces; ++i)
+            items[full_at + i] = make_int4(r, first + i * p.size, first + (i + 1) * p.size, part + i);
+    }
+    items[base[p.last] + last_at] =
+        make_int4(r, first + p.degree - p.last, first + p.degree, p.pieces > 1 ? part + p.pieces - 1 : -1);
+}
+
 }  // namespace tango
 
 using namespace tango;
 
 extern "C" {
+
+size_t tango_attention_items_workspace(void) { return sizeof(ItemCounts); }
+
+int tango_attention_items(int32_t* items, int32_t* split, const int64_t* indptr, int64_t rows, int64_t num_edges, int64_t cap,
+                          void* counts, size_t counts_bytes, tango_stream_t stream) {
+    if (rows < 0 || num_edges < 0 || cap < 1) return TANGO_ERR_INVALID_ARG;
+    if (cap >= kLengths || rows >= (1LL << 31) || num_edges > (1LL << 30) || rows + num_edges / cap >= (1LL << 31))
+        return TANGO_ERR_UNSUPPORTED;
+    if (!counts || counts_bytes < sizeof(ItemCounts) || !aligned_to(counts, 16)) return TANGO_ERR_WORKSPACE;
+    if (rows == 0) return TANGO_OK;
+    if (!items || !indptr || !aligned_to(items, 16) || !aligned_to(split, 16) || (num_edges > cap && !split)) return TANGO_ERR_INVALID_ARG;
+    ItemCounts* c = static_cast<ItemCounts*>(counts);
+    const dim3 grid(static_cast<uint32_t>(ceil_div(rows, 256))), block(256);
+    hipStream_t s = as_stream(stream);
+    hipLaunchKernelGGL(items_count_kernel, grid, block, 0, s, c, indptr, rows, static_cast<int>(cap));
+    hipLaunchKernelGGL(items_scan_kernel, dim3(1), dim3(64), 0, s, c);
+    hipLaunchKernelGGL(items_place_kernel, grid, block, 0, s, reinterpret_cast<int4*>(items), reinterpret_cast<int4*>(split), c, indptr,
+                       rows, static_cast<int>(cap));
+    return launch_status();
+}
 
 size_t tango_graph_attention_workspace(const tango_attention* t, const tango_attn_items* by_dst, const tango_attn_items* by_src,
                                        int masked) {

@@ -27,48 +27,30 @@ def item_edges(edges):
     return cap
 
 
-# Rows up to which the items are computed on the host: some thirty small operations and three counts read back take the
-# device 370 to 400 us whatever the size, the host 260 us at 2000 rows and 650 us at 8000.
-HOST_ROWS = 2048
-
-
 class AttentionItems:
-    """One orientation of a graph cut into work items (``tango_attn_items`` of include/tango_hip.h)."""
+    """One orientation of a graph cut into work items (``tango_attn_items`` of include/tango_hip.h) on its device."""
 
     def __init__(self, indptr, indices, edge_ids, cap=None):
         cap = item_edges(indices.numel()) if cap is None else cap
-        device = indptr.device
-        rows = indptr.numel() - 1
-        if rows <= HOST_ROWS:
-            indptr = indptr.cpu()
-        dev = indptr.device
-        first_slot, last_slot = indptr[:-1], indptr[1:]
-        degree = last_slot - first_slot
-        pieces = torch.clamp((degree + (cap - 1)) // cap, min=1)
-        row = torch.repeat_interleave(torch.arange(rows, device=dev), pieces)
-        nth = torch.arange(row.numel(), device=dev) - (torch.cumsum(pieces, 0) - pieces)[row]
-        size = ((degree + pieces - 1) // pieces)[row]
-        first = first_slot[row] + nth * size
-        last = torch.minimum(first + size, last_slot[row])
-        cut = pieces[row] > 1
-        part = torch.where(cut, torch.cumsum(cut, 0) - 1, -1)
-        order = torch.sort(last - first, descending=True, stable=True).indices
-        items = torch.stack([row, first, last, part], 1)[order].to(torch.int32)
-        split = torch.nonzero(pieces > 1).flatten()
-        ends = torch.cumsum(pieces[split], 0)
-        split_items = torch.stack([split, ends - pieces[split], ends, torch.zeros_like(split)], 1).to(torch.int32)
-        self.items, self.split = items.to(device).contiguous(), split_items.to(device).contiguous()
+        device, rows, edges = indptr.device, indptr.numel() - 1, indices.numel()
+        items = torch.empty((rows + edges // cap, 4), dtype=torch.int32, device=device)
+        split = torch.empty((edges // cap, 4), dtype=torch.int32, device=device)
+        nbytes = _L.tango_attention_items_workspace()
+        counts = torch.zeros(nbytes // 4, dtype=torch.int32, device=device)
+        check(_L.tango_attention_items(_ptr(items), _ptr(split), _ptr(indptr), rows, edges, cap, _ptr(counts), nbytes, _stream()),
+              "attention_items")
+        num_split, num_parts = counts[:2].tolist()  # waits for the kernels: any stream may use the items from here on
+        self.items, self.split = items[:rows - num_split + num_parts], split[:num_split]
         self.indices, self.edge_ids = indices, edge_ids
         s = _lib.AttnItems()
-        s.num_items, s.num_split, s.num_edges = self.items.size(0), self.split.size(0), indices.numel()
-        s.num_parts = int(ends[-1]) if ends.numel() else 0
+        s.num_items, s.num_split, s.num_parts, s.num_edges = self.items.size(0), num_split, num_parts, edges
         s.items, s.split, s.indices, s.edge_ids = _ptr(self.items), _ptr(self.split), _ptr(indices), _ptr(edge_ids)
         self.struct, self.ref = s, ctypes.byref(s)
 
 
 def _items(graph, orientation):
     """The items of a preprocessed graph, built once per orientation and kept on the graph with the index arrays they
-    were built from.  Building sorts on the device and reads counts back, so it cannot happen inside a capture."""
+    were built from.  Building reads two counts back, so it cannot happen inside a capture."""
     fmt, narrow, ordered = (("adj_csc", "adj_csc32", "csc_slots_are_edge_ids") if orientation == "in" else
                             ("adj_csr", "adj_csr32", "csr_slots_are_edge_ids"))
     if not hasattr(graph, narrow):
@@ -80,7 +62,6 @@ def _items(graph, orientation):
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("graph_attention: run prepare_attention(graph) before capturing")
     items = AttentionItems(indptr, narrow[0], None if getattr(graph, ordered) else narrow[1])
-    torch.cuda.current_stream(indptr.device).synchronize()  # other streams may use the items from here on
     setattr(graph, "_attention_items_" + orientation, (indptr, narrow, items))
     return items
 

@@ -82,28 +82,15 @@ def test_attention_backward_abi_refusals():
     assert L.tango_graph_attention_workspace(refs[0], refs[1], refs[1], 0) >= 4 * 2 * 8  # two floats a destination and head
 
 
-@pytest.mark.parametrize("cap", [1, 3, 64])
-def test_items_cover_every_edge_once(cap):
-    """The cut into items: every slot once, rows in slot order, no item longer than the cap, empty rows present."""
-    from tango_amd.graph_attention import AttentionItems
-    degree = torch.tensor([0, 1, 200, 0, 64, 65, 3, 0, 129, 2])
-    indptr = torch.zeros(11, dtype=torch.int64)
-    indptr[1:] = torch.cumsum(degree, 0)
-    a = AttentionItems(indptr, torch.zeros(int(indptr[-1]), dtype=torch.int32), None, cap=cap)
-    items = a.items.tolist()
-    lengths = [last - first for _, first, last, _ in items]
-    assert lengths == sorted(lengths, reverse=True) and max(lengths) <= cap
-    seen = torch.zeros(int(indptr[-1]), dtype=torch.int64)
-    for row, first, last, part in items:
-        assert indptr[row] <= first <= last <= indptr[row + 1]
-        seen[first:last] += 1
-    assert (seen == 1).all() and sorted({r for r, _, _, _ in items}) == list(range(10))
-    cut = {row: (a0, a1) for row, a0, a1, _ in a.split.tolist()}
-    for row in range(10):
-        mine = sorted(i for i in items if i[0] == row)
-        if row not in cut:
-            assert len(mine) == 1 and mine[0][3] == -1
-        else:
-            assert [i[3] for i in mine] == list(range(*cut[row])) and mine[0][1] == indptr[row] and mine[-1][2] == indptr[row + 1]
-            assert all(x[2] == y[1] for x, y in zip(mine, mine[1:]))
-    assert a.struct.num_parts == sum(b - c for c, b in cut.values())
+def test_items_abi_refusals():
+    from tango_amd import _lib
+    L = _lib.lib()
+    n = L.tango_attention_items_workspace()
+    assert L.tango_attention_items(16, 16, 16, 4, 5, 0, 16, n, None) == -1
+    assert L.tango_attention_items(16, 16, 16, 4, 5, 513, 16, n, None) == -2
+    assert L.tango_attention_items(16, 16, 16, 1 << 31, 5, 8, 16, n, None) == -2
+    assert L.tango_attention_items(16, 16, 16, 4, (1 << 30) + 1, 8, 16, n, None) == -2
+    assert L.tango_attention_items(16, 16, 16, 4, 5, 8, 16, n - 1, None) == -4
+    assert L.tango_attention_items(16, None, 16, 4, 9, 8, 16, n, None) == -1
+    assert L.tango_attention_items(20, 16, 16, 4, 9, 8, 16, n, None) == -1
+    assert L.tango_attention_items(None, None, None, 0, 0, 8, 16, n, None) == 0

@@ -95,6 +95,41 @@ def run(graph, q, k, v, dout, **kw):
     return [out, *torch.autograd.grad(out, leaves, dout)]
 
 
+@pytest.mark.parametrize("cap", [1, 3, 16, 64, 512])
+@pytest.mark.parametrize("rows", [1, 10, 255, 256, 257, 5000])
+def test_items_cover_every_edge_once(rows, cap):
+    """The cut into items: every slot once, rows in slot order, no item longer than the cap, longest first, empty rows
+    present, parts of a row consecutive."""
+    from tango_amd.graph_attention import AttentionItems
+    gen = torch.Generator().manual_seed(rows + cap)
+    degree = (torch.rand(rows, generator=gen) ** 6 * 2000).long()
+    degree[:10] = torch.tensor([0, 1, 200, 0, 64, 65, 3, 0, 129, 2])[:rows]
+    indptr = torch.zeros(rows + 1, dtype=torch.int64)
+    indptr[1:] = torch.cumsum(degree, 0)
+    a = AttentionItems(indptr.cuda(), torch.zeros(int(indptr[-1]), dtype=torch.int32, device="cuda"), None, cap=cap)
+    items, split = a.items.cpu().long(), a.split.cpu().long()
+    lengths = items[:, 2] - items[:, 1]
+    assert (lengths[:-1] >= lengths[1:]).all() and int(lengths.max()) <= cap and int(lengths.min()) >= 0
+    pieces = torch.clamp((degree + cap - 1) // cap, min=1)
+    assert torch.equal(torch.bincount(items[:, 0], minlength=rows), pieces)
+    order = torch.argsort(items[:, 0] * (int(indptr[-1]) + 1) + items[:, 1], stable=True)
+    items = items[order]
+    starts = torch.cumsum(pieces, 0) - pieces
+    assert torch.equal(items[starts, 1], indptr[:-1]) and torch.equal(items[starts + pieces - 1, 2], indptr[1:])
+    inner = torch.ones(len(items), dtype=torch.bool)
+    inner[starts] = False
+    assert torch.equal(items[1:, 1][inner[1:]], items[:-1, 2][inner[1:]])
+    cut = torch.nonzero(pieces > 1).flatten()
+    assert sorted(split[:, 0].tolist()) == cut.tolist() and a.struct.num_parts == int(pieces[cut].sum())
+    parts = torch.full((rows,), -1)
+    parts[split[:, 0]] = split[:, 1]
+    assert torch.equal(split[:, 2] - split[:, 1], pieces[split[:, 0]])
+    nth = torch.arange(len(items)) - starts[items[:, 0]]
+    assert torch.equal(items[:, 3], torch.where(pieces[items[:, 0]] > 1, parts[items[:, 0]] + nth, -1))
+    taken = torch.sort(items[items[:, 3] >= 0, 3]).values
+    assert torch.equal(taken, torch.arange(a.struct.num_parts))
+
+
 @pytest.mark.parametrize("t", sorted(TYPES))
 @pytest.mark.parametrize("dim", [1, 2, 3, 4, 7, 8, 12, 16, 24, 31, 32, 40, 64, 72, 100, 128, 136, 250, 256])
 def test_dims(dim, t):
