@@ -214,12 +214,14 @@ __device__ __forceinline__ float log2_total(float m, float l) { return l == 0.0f
 // Forward at 2 / 4 / 6 / 8: 424 / 413 / 391 / 387 us ([169343, 8, 32] fp32, 1.3 M edges), 577 / 552 / 553 / 605 us (5.3 M
 // edges, heads 8 over 2).  dq: 456 / 430 / 425 / 422 us, from checkpoints [169343, 4, 64] 197 / 225 / 235 / 213 us;
 // dk, dv: 489 / 486 / 492 / 541 us, from checkpoints 310 / 315 / 351 / 532 us.
-constexpr int kForwardEdges = 6;
+// Rows that no vector divides take four forward: the masks of six cost more registers ([169343, 3, 250] fp16: 730 us
+// against 790 us).
+constexpr int forward_edges(int mode) { return mode == kWhole ? 6 : 4; }
 constexpr int backward_edges(bool scaled) { return scaled ? 2 : 4; }
 
 template <typename T, int VEC, int LPH, int MODE>
 __global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnArgs a) {
-    constexpr int U = kForwardEdges;
+    constexpr int U = forward_edges(MODE);
     const ItemLane L = item_lane<LPH>(a, a.heads);
     if (!L.on) return;
     const RowLane<VEC, LPH, MODE> lane(L.j, a.dim);
