@@ -13,10 +13,10 @@
 //   dk, dv    one pass over a source's out-edges: p = 2^(logit - log2 denominator), dv[s] += p dout[d],
 //             dk[s] += scale p (dp - delta) q[d]; over all query heads that share the key head.
 //
-// Work items.  A row (destination or source) with its edges is cut into items of at most kItemEdges edges; items are
+// Work items.  A row (destination or source) with its edges is cut into items of at most 16 .. 512 edges; items are
 // sorted by length, longest first, so that the items of a wavefront end together and the launch has no long tail.  A
 // row that is one item is finished by its owner; rows of several items leave partial results that a join kernel adds
-// in item order: nothing here depends on scheduling, and there are no atomics.
+// in item order: no result depends on scheduling, and no sum is made with atomics.
 //
 // Lanes.  An item and a tile of heads belong to G lanes: LPH lanes for each head, VEC elements (16 bytes of the
 // gathered type) each, and as many neighbouring heads as bring the gathered piece of a row to 256 bytes, two lines of L2
@@ -83,8 +83,8 @@ __device__ __forceinline__ float lanes_sum(float x) {
 //   kWhole    dim is a multiple of VEC and every row starts on a vector: elements j VEC .. j VEC + VEC - 1.
 //   kShifted  any dim >= VEC, any alignment: the same, except that the last lane with elements is moved back to end with
 //             the row, so that every load is one whole vector inside the row.  What it then shares with its neighbour
-//             is masked to zero.  (dim 250 in fp16: 600 us a pass at [169343, 3, 250] and 1.3 M edges instead of 1800 us
-//             with a load per element.)
+//             is masked to zero.  (dim 250 in fp16, [169343, 3, 250] and 1.3 M edges: forward 746 us instead of 1800 us with
+//             a load per element.)
 //   kSingle   dim < VEC: one lane, a load per element.
 enum RowMode { kWhole, kShifted, kSingle };
 
@@ -164,7 +164,7 @@ __device__ __forceinline__ void store_part(float* head, const RowLane<VEC, LPH, 
 struct ItemLane {
     int4 it;  // row, first slot, last slot + 1, part
     int head, j;
-    bool item, on;  // a real item; and a real head
+    bool on;  // a real item and a real head
 };
 
 template <int LPH>
@@ -179,9 +179,8 @@ __device__ __forceinline__ ItemLane item_lane(const AttnArgs& a, int heads) {
     const int64_t id = block * (256 >> g_log) + (threadIdx.x >> g_log);
     r.head = (tile << a.tile_log) + gl / LPH;
     r.j = gl & (LPH - 1);
-    r.item = id < a.num_items;
-    r.on = r.item && r.head < heads;
-    r.it = r.item ? a.items[id] : make_int4(0, 0, 0, -1);
+    r.on = id < a.num_items && r.head < heads;
+    r.it = r.on ? a.items[id] : make_int4(0, 0, 0, -1);
     return r;
 }
 

@@ -445,6 +445,48 @@ def test_on_another_stream():
     assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, here))
 
 
+def test_two_streams_at_once():
+    """Calls on two streams in flight together, each with rows that leave parts in its scratch."""
+    rng = np.random.default_rng(43)
+    src, dst = powerlaw_graph(rng, 600, 60_000)
+    g = make_graph(src, dst, 600, 600)
+    cases = [(inputs(600, 600, 4, 2, 32, torch.float32, seed=s), kw) for s, kw in ((1, {}), (2, dict(checkpoint="int8")))]
+    want = [run(g, *x, **kw) for x, kw in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = []
+        for s, (x, kw) in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(run(g, *x, **kw))
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(u, w) for u, w in zip(a, b))
+
+
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_offsets_beyond_32_bits(checkpoint):
+    """Keys and values of more than 2^31 elements, read and written at both ends."""
+    n, D = 8_500_000, 256
+    assert n * D > 1 << 31
+    src = torch.tensor([0, 1, n - 1, n - 2, n - 1, 5, n // 2, n - 3])
+    dst = torch.tensor([0, 0, 0, 1, 1, 1, 2, 2])
+    g = make_graph(src, dst, n, 3)
+    used = torch.unique(src)
+    small = torch.searchsorted(used, src)
+    x = inputs(len(used), 3, 1, 1, D, torch.bfloat16, seed=3)
+    k, v = (torch.zeros(n, 1, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    k[used.cuda()], v[used.cuda()] = x[1], x[2]
+    got = run(g, x[0], k, v, x[3], checkpoint=checkpoint)
+    h = make_graph(small, dst, len(used), 3)
+    want = run(h, *x, checkpoint=checkpoint)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for a, b in zip(got[2:], want[2:]):
+        assert torch.equal(a[used.cuda()], b)
+        a[used.cuda()] = 0
+        assert not a.any()
+
+
 def test_a_graph_preprocessed_again_gets_new_items():
     from tango_amd.graph import Graph
     from tango_amd.graph_attention import graph_attention

@@ -106,6 +106,54 @@ def test_same_bits_every_time():
     assert torch.equal(first[0], weight_grad(dy, p))
 
 
+def test_captured_and_replayed():
+    """A checkpoint and its weight gradient in one HIP graph, replayed over new inputs with eager work in between."""
+    from tango_amd.checkpoint import pack, weight_grad
+    dy, x = make(3000, 40, 96, "fp32", seed=2)
+    weight_grad(dy, pack(x, 32), True)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        dw, db = weight_grad(dy, pack(x, 32), True)
+    for seed in range(3):
+        for a, b in zip((dy, x), make(3000, 40, 96, "fp32", seed=10 + seed)):
+            a.copy_(b)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((dw, db), weight_grad(dy, pack(x, 32), True)))
+
+
+def test_two_streams_at_once():
+    from tango_amd.checkpoint import pack, weight_grad
+    cases = [make(20_000, 64, 130, t, seed=s) for s, t in ((1, "fp32"), (2, "bf16"))]
+    packed = [pack(x, 64) for _, x in cases]
+    want = [weight_grad(dy, p, True) for (dy, _), p in zip(cases, packed)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = []
+        for s, (dy, _), p in zip(streams, cases, packed):
+            with torch.cuda.stream(s):
+                got.append(weight_grad(dy, p, True))
+        torch.cuda.synchronize()
+        assert all(torch.equal(u, w) for a, b in zip(want, got) for u, w in zip(a, b))
+
+
+def test_offsets_beyond_32_bits():
+    """Rows whose elements lie past 2^31 in both operands: zeros but for the first and the last rows."""
+    from tango_amd.checkpoint import pack, weight_grad
+    M, N, K = 8_500_000, 256, 256
+    assert M * N > 1 << 31
+    dy, x = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda"), torch.zeros(M, K, dtype=torch.bfloat16, device="cuda")
+    a, b = make(400, N, K, "bf16", seed=6)
+    for whole, part in ((dy, a), (x, b)):
+        whole[:200], whole[-200:] = part[:200], part[200:]
+    p, q = pack(x, 64), pack(b, 64)
+    del x
+    assert torch.equal(p.values[-200:], q.values[200:]) and torch.equal(p.scale[-200:], q.scale[200:])
+    compare(a, q, "bf16", weight_grad(dy, p, True))
+
+
 def test_no_rows_and_no_columns():
     from tango_amd.checkpoint import pack, weight_grad
     z = lambda *s: torch.zeros(*s, device="cuda")
