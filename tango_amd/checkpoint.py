@@ -58,7 +58,7 @@ class Packed:
         return self.values.size(0) * self.values.stride(0) + 4 * self.scale.numel() if self.values.numel() else 0
 
 
-def _rows_of(x):
+def rows_of(x):
     """[rows, cols] with contiguous columns: a view where x's layout allows one."""
     cols = x.size(-1)
     rows = math.prod(x.shape[:-1])
@@ -91,7 +91,7 @@ def pack(x, group=None):
         raise ValueError("pack: group must be a positive whole number of columns")
     group = int(group)
     with on_device_of(x):
-        flat = _rows_of(x.detach())
+        flat = rows_of(x.detach())
         scale = torch.empty((flat.size(0), -(-cols // group)), dtype=torch.float32, device=x.device)
         values = pack_rows(flat, group, scale)
     return Packed(values, scale, group, x.shape, x.dtype)
@@ -127,7 +127,7 @@ def weight_grad(dy, packed, want_bias=False):
     if math.prod(dy.shape[:-1]) != rows:
         raise RuntimeError("weight_grad: dy needs a row for each of the checkpoint's %d" % rows)
     with on_device_of(dy):
-        flat = _rows_of(dy.detach())
+        flat = rows_of(dy.detach())
         if rows == 0:
             dw, db = flat.new_zeros((n, cols)), flat.new_zeros(n)
         else:

@@ -12,7 +12,7 @@ import torch
 from torch.autograd.function import Function, once_differentiable
 
 from . import _lib
-from .checkpoint import DTYPES, need_float, on_device_of, pack_rows
+from .checkpoint import DTYPES, need_float, on_device_of, pack_rows, rows_of
 from .kernels import _L, _ptr, _stream, _workspace, check, refuse_capture
 
 
@@ -84,7 +84,7 @@ def _hold(q, k, v):
     lie side by side, since the backward pass reads them together."""
     scales = [torch.empty(q.shape[:2] + (1,), dtype=torch.float32, device=q.device),
               torch.empty(k.shape[:2] + (2,), dtype=torch.float32, device=q.device)]
-    flat = [x.reshape(x.size(0), x.size(1) * x.size(2)) for x in (q, k, v)]
+    flat = [rows_of(x.flatten(1)) for x in (q, k, v)]  # of heads of one column, the columns may lie apart
     held = [pack_rows(x, q.size(2), s) for x, s in zip(flat, (scales[0][..., 0], scales[1][..., 0], scales[1][..., 1]))]
     return held, scales
 

@@ -320,6 +320,26 @@ def test_strides(t):
     check([want[0], *grads], want, bound, t)
 
 
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+@pytest.mark.parametrize("layout", ["transposed", "broadcast", "sliced"])
+def test_heads_of_one_column(layout, checkpoint):
+    """Heads of one column whose heads lie apart, or on each other: held and attended as their contiguous copies are."""
+    from tango_amd.graph_attention import graph_attention
+    n, H = 50, 6
+    gen = torch.Generator().manual_seed(8)
+    make = {"transposed": lambda: torch.randn(H, n, 1, generator=gen).cuda().transpose(0, 1),
+            "broadcast": lambda: torch.randn(n, 1, 1, generator=gen).cuda().expand(n, H, 1),
+            "sliced": lambda: torch.randn(n, H, 3, generator=gen).cuda()[:, :, 1:2]}[layout]
+    g = make_graph(torch.randint(0, n, (400,), generator=gen), torch.randint(0, n, (400,), generator=gen), n, n)
+    results = []
+    x = [make() for _ in range(3)]
+    dout = torch.randn(n, H, 1, generator=gen).cuda()
+    for leaves in ([t.detach().requires_grad_() for t in x], [t.contiguous().requires_grad_() for t in x]):
+        out = graph_attention(g, *leaves, checkpoint=checkpoint)
+        results.append([out.detach(), *torch.autograd.grad(out, leaves, dout)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 def test_gradients_of_shared_and_broadcast_leaves():
     """One leaf for keys and values, one row of queries for every destination: autograd adds what belongs together."""
     from tango_amd.graph_attention import graph_attention
