@@ -155,20 +155,23 @@ class checkpoint_linear(Function):
             if t.dtype != x.dtype or t.device != x.device:
                 raise RuntimeError("checkpoint_linear: %s must have x's type and device" % name)
         ctx.has_bias = bias is not None
-        ctx.held = pack(x, group) if ctx.needs_input_grad[1] else None
-        ctx.save_for_backward(weight if ctx.needs_input_grad[0] else None)
+        held = pack(x, group) if ctx.needs_input_grad[1] else None
+        # saved and not kept on ctx: released with the backward pass, as what other layers save is
+        ctx.held = held and (held.group, held.shape, held.dtype)
+        ctx.save_for_backward(weight if ctx.needs_input_grad[0] else None, *((held.values, held.scale) if held else ()))
         return F.linear(x, weight, bias)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         refuse_capture("checkpoint_linear.backward")
-        weight, = ctx.saved_tensors
+        weight, *held = ctx.saved_tensors
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
         dx = torch.matmul(dy, weight) if want_x else None
         dw = db = None
         if want_w:
-            dw, db = weight_grad(dy, ctx.held, True) if want_b else (weight_grad(dy, ctx.held), None)
+            held = Packed(*held, *ctx.held)
+            dw, db = weight_grad(dy, held, True) if want_b else (weight_grad(dy, held), None)
         elif want_b:
             db = dy.float().reshape(-1, dy.size(-1)).sum(0).to(dy.dtype)
         return dx, dw, db, None

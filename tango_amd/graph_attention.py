@@ -86,7 +86,7 @@ def _hold(q, k, v):
               torch.empty(k.shape[:2] + (2,), dtype=torch.float32, device=q.device)]
     flat = [rows_of(x.flatten(1)) for x in (q, k, v)]  # of heads of one column, the columns may lie apart
     held = [pack_rows(x, q.size(2), s) for x, s in zip(flat, (scales[0][..., 0], scales[1][..., 0], scales[1][..., 1]))]
-    return held, scales
+    return (*held, *scales)
 
 
 def _struct(q, k, v, scale):
@@ -97,11 +97,9 @@ def _struct(q, k, v, scale):
                           None, None, None, 0, 0, 0, 0, scale)
 
 
-def _struct_held(q_shape, k_shape, dtype, held, scales, scale):
+def _struct_held(q_shape, k_shape, dtype, q, k, v, q_scale, kv_scale, scale):
     """tango_attention of their 8-bit forms."""
     (n, heads, dim), (m, kv_heads, _) = q_shape, k_shape
-    q, k, v = held
-    q_scale, kv_scale = scales
     at = _ptr(kv_scale)
     return _lib.Attention(n, m, heads, kv_heads, dim, DTYPES[dtype], 1, _ptr(q), _ptr(k), _ptr(v), q.stride(0), dim, k.stride(0), dim,
                           v.stride(0), dim, _ptr(q_scale), at, at + 4 if at else None, *q_scale.stride()[:2],
@@ -123,9 +121,8 @@ class _GraphAttention(Function):
             ctx.graph, ctx.scale, ctx.held = graph, scale, None
             if any(ctx.needs_input_grad[1:4]):
                 if checkpoint:
-                    ctx.held = _hold(q, k, v)
-                    ctx.shapes = q.shape, k.shape, q.dtype
-                    ctx.save_for_backward(edge_mask)
+                    ctx.held = q.shape, k.shape, q.dtype
+                    ctx.save_for_backward(edge_mask, *_hold(q, k, v))
                 else:
                     ctx.save_for_backward(edge_mask, q, k, v)
         return out
@@ -136,14 +133,14 @@ class _GraphAttention(Function):
         refuse_capture("graph_attention.backward")
         with on_device_of(dout):
             by_dst, by_src = _items(ctx.graph, "in"), _items(ctx.graph, "out")
-            edge_mask, *qkv = ctx.saved_tensors
+            edge_mask, *kept = ctx.saved_tensors
             dout = _unit_last(dout)
             if ctx.held is None:
-                t = _struct(*qkv, ctx.scale)
-                q_shape, k_shape = qkv[0].shape, qkv[1].shape
+                t = _struct(*kept, ctx.scale)
+                q_shape, k_shape = kept[0].shape, kept[1].shape
             else:
-                q_shape, k_shape, dtype = ctx.shapes
-                t = _struct_held(q_shape, k_shape, dtype, *ctx.held, ctx.scale)
+                q_shape, k_shape, dtype = ctx.held
+                t = _struct_held(q_shape, k_shape, dtype, *kept, ctx.scale)
             grads = [torch.empty(shape, dtype=dout.dtype, device=dout.device) if need else None
                      for shape, need in zip((q_shape, k_shape, k_shape), ctx.needs_input_grad[1:4])]
             ref = ctypes.byref(t)

@@ -519,6 +519,24 @@ def test_a_graph_preprocessed_again_gets_new_items():
     assert torch.equal(out[0], v[3]) and (out[2] == 0).all()
 
 
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_kept_tensors_are_released_by_the_backward_pass(checkpoint):
+    from tango_amd.graph_attention import graph_attention, prepare_attention
+    # prepared, so that the backward pass leaves no new items (16 bytes a row) on the graph
+    g = prepare_attention(make_graph(torch.arange(4000), torch.arange(4000), 4000, 4000))
+    leaf = torch.randn(4000, 8, 32, device="cuda", requires_grad=True)
+    q, k, v = (leaf * c for c in (1.0, 2.0, 3.0))  # nothing but the attention needs them
+    out = graph_attention(g, q, k, v, checkpoint=checkpoint)
+    del q, k, v
+    loss = out.sum()
+    before = torch.cuda.memory_allocated()
+    loss.backward()
+    # the gradient is new; all that was kept (a byte an element at least) is gone
+    assert torch.cuda.memory_allocated() - before <= leaf.numel() * (4 - 3 * (1 if checkpoint else 4)) + 16384
+    with pytest.raises(RuntimeError, match="second time"):
+        loss.backward()
+
+
 def test_refusals():
     from tango_amd.graph import Graph
     from tango_amd.graph_attention import graph_attention

@@ -186,6 +186,22 @@ def test_linear_layer():
     torch.autograd.grad(bare(x.detach()).sum(), bare.weight)
 
 
+def test_held_input_is_released_by_the_backward_pass():
+    """As what torch saves is: an output that lives on keeps nothing, and a second backward pass is refused."""
+    from tango_amd.checkpoint import CheckpointLinear
+    layer = CheckpointLinear(512, 8).cuda()
+    x = torch.randn(4096, 512, device="cuda")
+    before = torch.cuda.memory_allocated()
+    y = layer(x)
+    kept = torch.cuda.memory_allocated() - before
+    loss = y.sum()
+    loss.backward()
+    small = 4 * (y.numel() + 512 * 8 + 8) + 16384  # y and the gradients, and rounding up
+    assert kept > x.numel() and torch.cuda.memory_allocated() - before < small < x.numel()
+    with pytest.raises(RuntimeError, match="second time"):
+        loss.backward()
+
+
 def test_refusals():
     from tango_amd.checkpoint import CheckpointLinear, checkpoint_linear, pack, weight_grad
     dy, x = make(10, 8, 16, "fp32")
