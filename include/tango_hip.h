@@ -632,7 +632,7 @@ typedef struct tango_attention {
     int64_t q_row, q_head, k_row, k_head, v_row, v_head;
     const float *q_scale, *k_scale, *v_scale;       /* of (row r, head h) at r * .._row + h * .._head (k, v: kv_..) */
     int64_t q_scale_row, q_scale_head, kv_scale_row, kv_scale_head;
-    float scale;
+    float scale;                                    /* 2^127 at most in size */
 } tango_attention;
 
 /* The rows of one orientation (destinations with their in-edges, or sources with their out-edges) as work items. */

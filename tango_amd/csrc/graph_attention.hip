@@ -1,5 +1,7 @@
 // C entries of the attention over a graph's edges: checks, workspace layout, the order of the passes.  The kernels are
 // in graph_attention.hpp.
+#include <math.h>
+
 #include "graph_attention.hpp"
 
 namespace tango {
@@ -27,6 +29,7 @@ static int check_shape(const tango_attention* t) {
     if (!t) return TANGO_ERR_INVALID_ARG;
     if (!float_type(t->dtype)) return TANGO_ERR_UNSUPPORTED;
     if (t->num_dst < 0 || t->num_src < 0 || t->heads <= 0 || t->kv_heads <= 0 || t->dim <= 0) return TANGO_ERR_INVALID_ARG;
+    if (!(fabsf(t->scale) <= 0x1p127f)) return TANGO_ERR_INVALID_ARG;  // times log2(e) it has to be finite
     if (t->num_dst >= (1LL << 31) || t->num_src >= (1LL << 31) || t->heads > 65536 || t->heads % t->kv_heads || t->dim > 256)
         return TANGO_ERR_UNSUPPORTED;
     return TANGO_OK;

@@ -193,6 +193,6 @@ def graph_attention(graph, q, k, v, scale=None, edge_mask=None, checkpoint=None)
     if checkpoint not in (None, "int8"):
         raise ValueError("graph_attention: checkpoint must be None or 'int8'")
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("graph_attention: scale must be finite")
+    if not abs(scale) <= 2.0 ** 127:  # times log2(e) it has to be finite in fp32
+        raise ValueError("graph_attention: scale must be finite, 2^127 at most")
     return _GraphAttention.apply(graph, q, k, v, scale, edge_mask, checkpoint == "int8")

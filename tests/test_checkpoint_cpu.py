@@ -68,6 +68,14 @@ def test_attention_abi_refusals(status, change):
     assert L.tango_graph_attention_fwd(16, ctypes.byref(t), ctypes.byref(i), None, None, 0, None) == status
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), 3e38, -3e38])
+def test_attention_scale_out_of_range(scale):
+    """Times log2(e), as the exponentials of base two take it, such a scale is not a finite fp32 number."""
+    L, t, i = _attention(scale=scale)
+    assert L.tango_graph_attention_fwd(16, ctypes.byref(t), ctypes.byref(i), None, None, 0, None) == -1
+    assert L.tango_graph_attention_workspace(ctypes.byref(t), ctypes.byref(i), None, 1) == 0
+
+
 def test_attention_backward_abi_refusals():
     L, t, i = _attention()
     refs = ctypes.byref(t), ctypes.byref(i)

@@ -519,6 +519,19 @@ def test_a_graph_preprocessed_again_gets_new_items():
     assert torch.equal(out[0], v[3]) and (out[2] == 0).all()
 
 
+def test_largest_scale():
+    """2^127 is taken, with queries that bring the logits back; what times log2(e) leaves fp32's range is refused."""
+    from tango_amd.graph_attention import graph_attention
+    q, k, v, dout = inputs(20, 20, 2, 2, 16, torch.float32)
+    g = make_graph(torch.arange(20).repeat(3), torch.arange(60) * 7 % 20, 20, 20)
+    # a power of two moved between the factors, which times log2(e) changes no bit
+    assert torch.equal(graph_attention(g, q * 2.0 ** -100, k, v, scale=2.0 ** 99), graph_attention(g, q, k, v, scale=0.5))
+    assert torch.isfinite(graph_attention(g, q * 2.0 ** -100, k * 2.0 ** -27, v, scale=2.0 ** 127)).all()
+    for scale in (1e39, -1e39, 3e38, 1e300):
+        with pytest.raises(ValueError):
+            graph_attention(g, q, k, v, scale=scale)
+
+
 @pytest.mark.parametrize("checkpoint", [None, "int8"])
 def test_kept_tensors_are_released_by_the_backward_pass(checkpoint):
     from tango_amd.graph_attention import graph_attention, prepare_attention
