@@ -58,6 +58,26 @@ class Packed:
         return self.values.size(0) * self.values.stride(0) + 4 * self.scale.numel() if self.values.numel() else 0
 
 
+def need_packed(packed, name):
+    """A checkpoint whose parts still fit each other and lie on one GPU: they can be replaced, or moved to the host."""
+    if not isinstance(packed, Packed):
+        raise TypeError("%s: expected what pack returned" % name)
+    values, scale, group = packed.values, packed.scale, packed.group
+    if values.dtype != torch.int8 or scale.dtype != torch.float32:
+        raise RuntimeError("%s: the checkpoint must hold int8 values and fp32 scales" % name)
+    if not values.is_cuda or values.device != scale.device:
+        raise RuntimeError("%s: the checkpoint must be on GPU" % name)
+    if not isinstance(group, int) or group < 1:
+        raise RuntimeError("%s: the checkpoint's group must be a positive whole number" % name)
+    *lead, cols = packed.shape
+    rows = math.prod(lead)
+    if values.shape != (rows, cols):
+        raise RuntimeError("%s: the checkpoint's values do not have its shape" % name)
+    if cols > 1 and values.stride(1) != 1 or scale.shape != (rows, -(-cols // group)) or not scale.is_contiguous():
+        raise RuntimeError("%s: the checkpoint must hold contiguous columns and a contiguous scale per row and run" % name)
+    return packed
+
+
 def rows_of(x):
     """[rows, cols] with contiguous columns: a view where x's layout allows one."""
     cols = x.size(-1)
@@ -100,8 +120,7 @@ def pack(x, group=None):
 def unpack(packed, dtype=None):
     """The tensor that ``packed`` stands for: value * scale in fp32, rounded to ``dtype`` (default: the type of the
     tensor that was packed)."""
-    if not isinstance(packed, Packed):
-        raise TypeError("unpack: expected what pack returned")
+    need_packed(packed, "unpack")
     dtype = packed.dtype if dtype is None else dtype
     if dtype not in DTYPES:
         raise RuntimeError("unpack: expected torch.float32, torch.bfloat16 or torch.float16 but got %s" % dtype)
@@ -118,8 +137,7 @@ def weight_grad(dy, packed, want_bias=False):
     layer's weight [out, in] and bias from the gradient ``dy`` [..., out] of its output, in dy's type, read straight
     from the 8-bit values.  Sums are fp32 in a fixed order."""
     need_float(dy, "dy")
-    if not isinstance(packed, Packed):
-        raise TypeError("weight_grad: expected what pack returned")
+    need_packed(packed, "weight_grad")
     if dy.dim() < 1 or dy.device != packed.device:
         raise RuntimeError("weight_grad: dy must be [..., out] on the checkpoint's device")
     rows, cols = packed.values.shape

@@ -17,6 +17,15 @@ def test_python_refusals():
         graph_attention(None, *(torch.zeros(2, 1, 4) for _ in range(3)))
 
 
+def test_checkpoints_on_the_host_are_refused():
+    from tango_amd.checkpoint import Packed, need_packed, unpack
+    p = Packed(torch.zeros(4, 16, dtype=torch.int8), torch.zeros(4, 2), 8, (4, 16), torch.float32)
+    with pytest.raises(RuntimeError, match="GPU"):
+        unpack(p)
+    with pytest.raises(TypeError):
+        need_packed(p.values, "unpack")
+
+
 def test_checkpoint_abi_refusals():
     from tango_amd import _lib
     L = _lib.lib()

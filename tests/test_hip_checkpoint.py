@@ -160,6 +160,23 @@ def test_on_another_stream():
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("change", [
+    dict(values=lambda p: p.values.cpu()), dict(scale=lambda p: p.scale.cpu()), dict(values=lambda p: p.values.float()),
+    dict(scale=lambda p: p.scale.double()), dict(scale=lambda p: p.scale[:, :2]), dict(scale=lambda p: p.scale.t().contiguous().t()),
+    dict(values=lambda p: p.values[:3]), dict(values=lambda p: p.values.t().contiguous().t()), dict(values=lambda p: p.values[:, :16]),
+    dict(group=lambda p: 0), dict(group=lambda p: 16), dict(group=lambda p: 8.0), dict(shape=lambda p: (5, 24)), dict(shape=lambda p: (4, 23)),
+])
+def test_altered_checkpoints_are_refused(change):
+    """A checkpoint whose parts were replaced or moved does not reach the kernels."""
+    from tango_amd.checkpoint import pack, unpack, weight_grad
+    p = pack(torch.randn(4, 24, device="cuda"), 8)
+    (name, make), = change.items()
+    setattr(p, name, make(p))
+    for call in (lambda: unpack(p), lambda: weight_grad(torch.ones(4, 3, device="cuda"), p)):
+        with pytest.raises(RuntimeError):
+            call()
+
+
 def test_refusals():
     from tango_amd.checkpoint import pack, unpack
     x = torch.randn(4, 8, device="cuda")
