@@ -168,6 +168,9 @@ class checkpoint_linear(Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, group=None):
+        if torch.is_autocast_enabled("cuda"):  # as F.linear does below, so that what is kept is what it ran on
+            to = torch.get_autocast_dtype("cuda")
+            x, weight, bias = (t.to(to) if isinstance(t, torch.Tensor) and t.dtype in DTYPES else t for t in (x, weight, bias))
         for t, name in ((x, "x"), (weight, "weight")) + (((bias, "bias"),) if bias is not None else ()):
             need_float(t, name)
             if t.dtype != x.dtype or t.device != x.device:

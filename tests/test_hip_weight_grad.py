@@ -186,6 +186,25 @@ def test_linear_layer():
     torch.autograd.grad(bare(x.detach()).sum(), bare.weight)
 
 
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+def test_linear_layer_under_autocast(t):
+    """Autocast runs the layer in its type on fp32 parameters; the gradients reach the parameters in theirs."""
+    from tango_amd.checkpoint import CheckpointLinear, pack
+    torch.manual_seed(4)
+    layer, plain = CheckpointLinear(96, 40, group=32).cuda(), torch.nn.Linear(96, 40).cuda()
+    plain.load_state_dict(layer.state_dict())
+    for x in (torch.randn(50, 96, device="cuda"), torch.randn(50, 96, device="cuda", dtype=TYPES[t])):
+        x.requires_grad_()
+        dy = torch.randn(50, 40, device="cuda", dtype=TYPES[t])
+        with torch.autocast("cuda", TYPES[t]):
+            y, z = layer(x), plain(x)
+        assert y.dtype == TYPES[t] and torch.equal(y, z)
+        dx, dw, db = torch.autograd.grad(y, (x, layer.weight, layer.bias), dy)
+        assert torch.equal(dx, torch.autograd.grad(z, x, dy)[0]) and dx.dtype == x.dtype
+        assert dw.dtype == db.dtype == torch.float32
+        compare(dy, pack(x.to(TYPES[t]), 32), t, (dw.to(TYPES[t]), db.to(TYPES[t])))
+
+
 def test_held_input_is_released_by_the_backward_pass():
     """As what torch saves is: an output that lives on keeps nothing, and a second backward pass is refused."""
     from tango_amd.checkpoint import CheckpointLinear
