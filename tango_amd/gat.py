@@ -181,6 +181,8 @@ class HGTLayer(nn.Module):
     instead: one pass, nothing kept per edge, probabilities formed again in the backward pass.  ``checkpoint="int8"``
     (with "recompute"): queries, keys and values are kept in 8 bits between the passes."""
 
+    attention, checkpoint = "quantized", None  # of layers that were pickled without them
+
     def __init__(self, in_dim, out_dim, n_heads, attention="quantized", checkpoint=None):
         super().__init__()
         if attention not in ("quantized", "recompute"):

@@ -41,11 +41,22 @@ class AttentionItems:
               "attention_items")
         num_split, num_parts = counts[:2].tolist()  # waits for the kernels: any stream may use the items from here on
         self.items, self.split = items[:rows - num_split + num_parts], split[:num_split]
-        self.indices, self.edge_ids = indices, edge_ids
+        self.indices, self.edge_ids, self.num_parts = indices, edge_ids, num_parts
+        self._point()
+
+    def _point(self):
         s = _lib.AttnItems()
-        s.num_items, s.num_split, s.num_parts, s.num_edges = self.items.size(0), num_split, num_parts, edges
-        s.items, s.split, s.indices, s.edge_ids = _ptr(self.items), _ptr(self.split), _ptr(indices), _ptr(edge_ids)
+        s.num_items, s.num_split, s.num_parts, s.num_edges = self.items.size(0), self.split.size(0), self.num_parts, self.indices.numel()
+        s.items, s.split, s.indices, s.edge_ids = _ptr(self.items), _ptr(self.split), _ptr(self.indices), _ptr(self.edge_ids)
         self.struct, self.ref = s, ctypes.byref(s)
+
+    def __getstate__(self):
+        """A graph is copied and saved with its items: without the addresses, which are the copy's own."""
+        return {name: value for name, value in self.__dict__.items() if name not in ("struct", "ref")}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._point()
 
 
 def _items(graph, orientation):
@@ -69,6 +80,8 @@ def _items(graph, orientation):
 def prepare_attention(graph):
     """Builds what ``graph_attention`` keeps with a preprocessed graph (the first call does it otherwise); needed
     before a forward pass is captured into a HIP graph."""
+    if not hasattr(graph, "adj_csc32"):
+        raise RuntimeError("graph_attention: the graph has not been through graph_preprocess")
     with on_device_of(graph.adj_csc[0]):
         _items(graph, "in")
         _items(graph, "out")

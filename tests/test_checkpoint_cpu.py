@@ -26,6 +26,24 @@ def test_checkpoints_on_the_host_are_refused():
         need_packed(p.values, "unpack")
 
 
+def test_preparing_a_graph_that_was_not_preprocessed():
+    from tango_amd.graph import Graph
+    from tango_amd.graph_attention import prepare_attention
+    with pytest.raises(RuntimeError, match="graph_preprocess"):
+        prepare_attention(Graph(torch.tensor([0]), torch.tensor([1]), 2, 2))
+
+
+def test_layers_pickled_without_an_attention():
+    from tango_amd.gat import HGTLayer
+    layer = HGTLayer(8, 8, 2)
+    state = layer.__dict__.copy()
+    for name in ("attention", "checkpoint"):
+        del state[name]
+    old = HGTLayer.__new__(HGTLayer)
+    old.__setstate__(state)
+    assert old.attention == "quantized" and old.checkpoint is None
+
+
 def test_checkpoint_abi_refusals():
     from tango_amd import _lib
     L = _lib.lib()

@@ -507,6 +507,21 @@ def test_offsets_beyond_32_bits(checkpoint):
         assert not a.any()
 
 
+def test_copied_and_saved_graphs(tmp_path):
+    """A graph is copied, and saved and loaded, with the items it keeps; they point at the copy's own arrays."""
+    import copy
+    from tango_amd.graph_attention import _items, prepare_attention
+    x = inputs(300, 300, 2, 2, 16, torch.float32)
+    g = prepare_attention(make_graph(*powerlaw_graph(np.random.default_rng(3), 300, 4000), 300, 300))
+    want = run(g, *x)
+    torch.save(g, tmp_path / "graph.pt")
+    for other in (copy.copy(g), copy.deepcopy(g), torch.load(tmp_path / "graph.pt", weights_only=False)):
+        kept = other._attention_items_in[2]
+        assert _items(other, "in") is kept and kept.struct.indices == other.adj_csc32[0].data_ptr()
+        got = run(other, *x)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 def test_a_graph_preprocessed_again_gets_new_items():
     from tango_amd.graph import Graph
     from tango_amd.graph_attention import graph_attention
