@@ -613,8 +613,8 @@ int tango_unpack_i8(void* x, int dtype, int64_t ldx, const int8_t* q, int64_t ld
    group as of tango_pack_i8; every row of q is readable to ldq.  ldq, group and q multiples of 4 are the fast case):
      dw[n, k] = sum_m dy[m, n] * (q[m, k] * scale[m, k / group]),   db[n] = sum_m dy[m, n]  (db may be NULL)
    for dy [M, N] (dtype, row stride ldy) and q [M, K], M <= 2^30, N and K <= 65536; dw [N, K] and db [N] in dtype, contiguous.  Sums are fp32 in a
-   fixed order; a row's dy * scale is held in three (fp32) or two (bf16, fp16) bf16 terms.  A dy that is not finite
-   gives a result that is not finite.  workspace: tango_weight_grad_i8_workspace bytes. */
+   fixed order; a row's dy * scale is held in three (fp32) or two (bf16, fp16) bf16 terms.  A dy that is not finite,
+   or whose product with the scale is not, gives a result that is not finite.  workspace: tango_weight_grad_i8_workspace bytes. */
 size_t tango_weight_grad_i8_workspace(int dtype, int64_t M, int64_t N, int64_t K, int64_t group);
 int tango_weight_grad_i8(void* dw, void* db, const void* dy, int dtype, int64_t ldy, const int8_t* q,
                          int64_t ldq, const float* scale, int64_t group, int64_t M, int64_t N, int64_t K,

@@ -135,7 +135,8 @@ def unpack(packed, dtype=None):
 def weight_grad(dy, packed, want_bias=False):
     """``dy.T @ x`` (and, with ``want_bias``, ``dy.sum(0)``) for the x that ``packed`` holds: the gradients of a linear
     layer's weight [out, in] and bias from the gradient ``dy`` [..., out] of its output, in dy's type, read straight
-    from the 8-bit values.  Sums are fp32 in a fixed order."""
+    from the 8-bit values.  Sums are fp32 in a fixed order.  Where dy, or dy times a row's scale, is not a finite fp32
+    number the result is not finite either (an infinity or a NaN)."""
     need_float(dy, "dy")
     need_packed(packed, "weight_grad")
     if dy.dim() < 1 or dy.device != packed.device:
