@@ -14,6 +14,7 @@ and values that way when asked to.
 """
 import contextlib
 import math
+import operator
 
 import torch
 import torch.nn as nn
@@ -43,38 +44,43 @@ def need_float(t, name):
 
 class Packed:
     """What ``pack`` returns: ``values`` int8 [rows, cols] (rows start 16-byte aligned), ``scale`` fp32
-    [rows, ceil(cols / group)], and the ``shape`` and ``dtype`` of the tensor it stands for."""
+    [rows, ceil(cols / group)], and the ``shape`` and ``dtype`` of the tensor it stands for.  Parts of a user's own
+    are checked here, once, and cannot be replaced afterwards."""
 
-    __slots__ = ("values", "scale", "group", "shape", "dtype")
+    __slots__ = ("_values", "_scale", "_group", "_shape", "_dtype")
+    values, scale, group, shape, dtype = (property(operator.attrgetter(name)) for name in __slots__)
 
     def __init__(self, values, scale, group, shape, dtype):
-        self.values, self.scale, self.group, self.shape, self.dtype = values, scale, group, tuple(shape), dtype
+        if values.dtype != torch.int8 or scale.dtype != torch.float32 or dtype not in DTYPES:
+            raise RuntimeError("Packed: values must be int8, the scale fp32, and dtype fp32, bf16 or fp16")
+        if not isinstance(group, int) or group < 1:
+            raise RuntimeError("Packed: group must be a positive whole number")
+        *lead, cols = shape
+        rows = math.prod(lead)
+        if values.shape != (rows, cols):
+            raise RuntimeError("Packed: the values do not have the tensor's shape")
+        if cols > 1 and values.stride(1) != 1 or scale.shape != (rows, -(-cols // group)) or not scale.is_contiguous():
+            raise RuntimeError("Packed: needs contiguous columns and a contiguous scale per row and run")
+        self._fill(values, scale, group, shape, dtype)
+
+    def _fill(self, values, scale, group, shape, dtype):
+        self._values, self._scale, self._group, self._shape, self._dtype = values, scale, group, tuple(shape), dtype
+        return self
 
     @property
     def device(self):
-        return self.values.device
+        return self._values.device
 
     def nbytes(self):
-        return self.values.size(0) * self.values.stride(0) + 4 * self.scale.numel() if self.values.numel() else 0
+        return self._values.size(0) * self._values.stride(0) + 4 * self._scale.numel() if self._values.numel() else 0
 
 
 def need_packed(packed, name):
-    """A checkpoint whose parts still fit each other and lie on one GPU: they can be replaced, or moved to the host."""
+    """A checkpoint on one GPU (it may have been saved and loaded elsewhere)."""
     if not isinstance(packed, Packed):
         raise TypeError("%s: expected what pack returned" % name)
-    values, scale, group = packed.values, packed.scale, packed.group
-    if values.dtype != torch.int8 or scale.dtype != torch.float32:
-        raise RuntimeError("%s: the checkpoint must hold int8 values and fp32 scales" % name)
-    if not values.is_cuda or values.device != scale.device:
+    if not packed._values.is_cuda or packed._scale.device != packed._values.device:
         raise RuntimeError("%s: the checkpoint must be on GPU" % name)
-    if not isinstance(group, int) or group < 1:
-        raise RuntimeError("%s: the checkpoint's group must be a positive whole number" % name)
-    *lead, cols = packed.shape
-    rows = math.prod(lead)
-    if values.shape != (rows, cols):
-        raise RuntimeError("%s: the checkpoint's values do not have its shape" % name)
-    if cols > 1 and values.stride(1) != 1 or scale.shape != (rows, -(-cols // group)) or not scale.is_contiguous():
-        raise RuntimeError("%s: the checkpoint must hold contiguous columns and a contiguous scale per row and run" % name)
     return packed
 
 
@@ -114,7 +120,7 @@ def pack(x, group=None):
         flat = rows_of(x.detach())
         scale = torch.empty((flat.size(0), -(-cols // group)), dtype=torch.float32, device=x.device)
         values = pack_rows(flat, group, scale)
-    return Packed(values, scale, group, x.shape, x.dtype)
+    return Packed.__new__(Packed)._fill(values, scale, group, x.shape, x.dtype)
 
 
 def unpack(packed, dtype=None):
@@ -192,7 +198,7 @@ class checkpoint_linear(Function):
         dx = torch.matmul(dy, weight) if want_x else None
         dw = db = None
         if want_w:
-            held = Packed(*held, *ctx.held)
+            held = Packed.__new__(Packed)._fill(*held, *ctx.held)
             dw, db = weight_grad(dy, held, True) if want_b else (weight_grad(dy, held), None)
         elif want_b:
             db = dy.float().reshape(-1, dy.size(-1)).sum(0).to(dy.dtype)

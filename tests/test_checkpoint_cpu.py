@@ -26,6 +26,25 @@ def test_checkpoints_on_the_host_are_refused():
         need_packed(p.values, "unpack")
 
 
+@pytest.mark.parametrize("change", [
+    dict(values=torch.zeros(4, 24)), dict(scale=torch.zeros(4, 3).double()), dict(scale=torch.zeros(4, 2)),
+    dict(scale=torch.zeros(3, 4).t()), dict(values=torch.zeros(3, 24, dtype=torch.int8)), dict(values=torch.zeros(24, 4, dtype=torch.int8).t()),
+    dict(values=torch.zeros(4, 16, dtype=torch.int8)), dict(group=0), dict(group=16), dict(group=8.0), dict(shape=(5, 24)),
+    dict(shape=(4, 23)), dict(dtype=torch.float64),
+])
+def test_checkpoints_of_parts_that_do_not_fit(change):
+    """A checkpoint put together by hand is checked, and its parts stay."""
+    from tango_amd.checkpoint import Packed
+    parts = dict(values=torch.zeros(4, 24, dtype=torch.int8), scale=torch.zeros(4, 3), group=8, shape=(2, 2, 24), dtype=torch.bfloat16)
+    p = Packed(**parts)
+    with pytest.raises(RuntimeError):
+        Packed(**{**parts, **change})
+    (name, value), = change.items()
+    with pytest.raises(AttributeError):
+        setattr(p, name, value)
+    assert getattr(p, name) is parts[name]
+
+
 def test_preparing_a_graph_that_was_not_preprocessed():
     from tango_amd.graph import Graph
     from tango_amd.graph_attention import prepare_attention

@@ -97,6 +97,21 @@ def test_kept_memory(graph):
     assert held["int8"] < held["recompute"]
 
 
+def test_kept_tensors_on_the_host(graph):
+    """torch's hooks on saved tensors see what is kept: offloaded to the host and back, the gradients are the same."""
+    from tango_amd.checkpoint import CheckpointLinear
+    from tango_amd.gat import HGTLayer
+    torch.manual_seed(9)
+    layer = HGTLayer(64, 64, 2, attention="recompute", checkpoint="int8").cuda()
+    proj = CheckpointLinear(64, 7, group=32).cuda()
+    x, dy = torch.randn(1500, 64, device="cuda"), torch.randn(1500, 7, device="cuda")
+    leaves = [*layer.parameters(), *proj.parameters()]
+    want = torch.autograd.grad(proj(layer(graph, x)), leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = proj(layer(graph, x))
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(y, leaves, dy)))
+
+
 def test_training_driver(capsys):
     from tango_amd.evaluation import train
     for checkpoint in (None, "int8"):
