@@ -97,7 +97,8 @@ def _hold(q, k, v):
     lie side by side, since the backward pass reads them together."""
     scales = [torch.empty(q.shape[:2] + (1,), dtype=torch.float32, device=q.device),
               torch.empty(k.shape[:2] + (2,), dtype=torch.float32, device=q.device)]
-    flat = [rows_of(x.flatten(1)) for x in (q, k, v)]  # of heads of one column, the columns may lie apart
+    # heads of one column may lie apart: those are copied, as all are that no view makes rows of
+    flat = [x.view(x.size(0), x.size(1) * x.size(2)) if x.is_contiguous() else rows_of(x.flatten(1)) for x in (q, k, v)]
     held = [pack_rows(x, q.size(2), s) for x, s in zip(flat, (scales[0][..., 0], scales[1][..., 0], scales[1][..., 1]))]
     return (*held, *scales)
 
